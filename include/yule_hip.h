@@ -48,6 +48,7 @@ extern "C" {
 #define YULE_DTYPE_Q5_K 13
 #define YULE_DTYPE_Q6_K 14
 #define YULE_DTYPE_Q8_K 15
+#define YULE_DTYPE_BF16 30 /* attention of batches only */
 
 typedef struct yule_hip_backend yule_hip_backend;
 typedef uint64_t yule_buffer;
@@ -222,6 +223,78 @@ int yule_hip_quantized_gemm_f32(yule_hip_backend *be, yule_buffer weights, yule_
 int yule_hip_quantized_gemm_noalloc(yule_hip_backend *be, yule_buffer weights, yule_buffer x_bf16,
                                     yule_buffer y, uint32_t m, uint32_t n_rows, uint32_t n_cols,
                                     uint32_t dtype);
+
+/* ---- batched serving (no counterpart in the trait, which has one sequence) ---- */
+
+/* Rows of a buffer: row r begins offset + r * stride elements (of the call's
+ * type) into it.  A slice of wider rows, such as the K part of one [q | k | v]
+ * product, is the same buffer with that row's width as the stride. */
+typedef struct {
+    yule_buffer buffer;
+    uint64_t offset, stride;
+} yule_rows;
+
+/* Causal attention with grouped heads over packed prompts: sequence s is rows
+ * offsets[s] .. offsets[s + 1] - 1 (u32[n_seqs + 1] on the device, not
+ * decreasing; a sequence may be empty), and for each of its rows r and query
+ * heads h (KV head g = h / (n_heads / n_kv_heads))
+ *   out[r, h] = sum_j softmax_j(q[r, h] . k[j, g] / sqrt(head_dim)) v[j, g],
+ * j from the sequence's first row to r.  q and out: n_rows rows of n_heads *
+ * head_dim, k and v: n_rows rows of n_kv_heads * head_dim.  Rows of out that
+ * belong to no sequence keep what they hold.  dtype: F32, F16 or BF16 for all
+ * four; scores, softmax and sums are f32 (16-bit types: each weight is rounded
+ * to the type for the product with v, and the result once).  A key that a row
+ * does not see has no influence on it, whatever it holds.  head_dim: a multiple
+ * of 8, at most 256.  Rows have to start at multiples of 16 bytes, strides be
+ * below 2^24 elements, and out be another buffer than the inputs; n_rows *
+ * n_heads / n_kv_heads < 2^31.  Offsets past n_rows or decreasing touch nothing
+ * outside the buffers, but which rows then hold results is not defined.
+ * Allocates nothing, and can be captured. */
+int yule_hip_prompt_attn(yule_hip_backend *be, const yule_rows *q, const yule_rows *k, const yule_rows *v,
+                         const yule_rows *out, yule_buffer offsets, uint32_t n_seqs, uint32_t n_rows,
+                         uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t dtype);
+
+/* Attention of the n_tokens (1..64) newest tokens of each of n_seqs sequences
+ * over a prefix that all of them share, read once for the batch, and each one's
+ * own tail: query row s * n_tokens + i sees prefix rows 0 .. prefix_len - 1 and
+ * the rows of tail s below tail_lens[s] - n_tokens + 1 + i (its own among them:
+ * the tail holds the n_tokens new rows last).  Tail s is rows s * tail_cap ..
+ * of k_tail and v_tail; tail_lens (u32[n_seqs] on the device) above tail_cap
+ * count as tail_cap.  A row that sees nothing gives zeros.  n_tokens above 1 is
+ * the step that scores drafted tokens.  prefix_len or tail_cap 0: that part's
+ * rows are not looked at and may be null; both at most 2^30.  Types, heads,
+ * alignment, aliasing and accuracy as for yule_hip_prompt_attn.  The chunks'
+ * results lie in the backend's workspace (it does not grow under capture: call
+ * once before with the same sizes). */
+int yule_hip_prefix_attn(yule_hip_backend *be, const yule_rows *q, const yule_rows *k_prefix, const yule_rows *v_prefix,
+                         uint32_t prefix_len, const yule_rows *k_tail, const yule_rows *v_tail, yule_buffer tail_lens,
+                         uint32_t tail_cap, const yule_rows *out, uint32_t n_seqs, uint32_t n_tokens,
+                         uint32_t n_heads, uint32_t n_kv_heads, uint32_t head_dim, uint32_t dtype);
+
+#define YULE_NO_TOKEN 0xFFFFFFFFu
+
+/* Verification of drafted tokens (the sampler's answer beyond argmax, for
+ * n_seqs requests at once).  Sequence s has draft_lens[s] drafts (u32[n_seqs],
+ * at most n_draft; handle 0: n_draft each), draft_tokens[s][i] (u32
+ * [n_seqs][n_draft]).  target: f32 rows s * (n_draft + 1) + i of vocab
+ * probabilities, of the token after i drafts; draft: rows s * n_draft + i, the
+ * probabilities that draft i was drawn from; uniforms: f32 [n_seqs][n_draft +
+ * 1] numbers in [0, 1).  Draft i is kept while all before it are and
+ * uniforms[i] * draft_i[x] < target_i[x]; the first that is not, a, is replaced
+ * by a token of weights max(target_a - draft_a, 0) (all zero: of target_a), and
+ * if all are kept one of target_a follows: the smallest token at which the
+ * running sum of the weights (f64) is above uniforms[n_draft] times their sum,
+ * else the last that has a weight.  accepted[s] = a; tokens[s][0 .. a] (u32
+ * [n_seqs][n_draft + 1]) the kept drafts and the new token, YULE_NO_TOKEN
+ * behind it.  Weights that are negative or NaN count as 0 (with none left the
+ * new token is YULE_NO_TOKEN); a draft of vocab or more is not kept.  n_draft 0
+ * (at most 1024): plain sampling, and draft, draft_tokens are not looked at.
+ * Outputs have to be other buffers than the inputs and each other.  Uses the
+ * backend's workspace, as yule_hip_prefix_attn. */
+int yule_hip_verify_drafts(yule_hip_backend *be, const yule_rows *target, const yule_rows *draft,
+                           yule_buffer draft_tokens, yule_buffer uniforms, yule_buffer draft_lens,
+                           yule_buffer accepted, yule_buffer tokens, uint32_t n_seqs, uint32_t n_draft,
+                           uint32_t vocab);
 
 /* ---- decode runner (yule-infer GpuTransformerRunner counterpart) ---- */
 

@@ -56,6 +56,10 @@ _SIGS: dict[str, tuple] = {
     "yule_hip_quantized_gemm": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint64] + [C.c_uint32] * 4),
     "yule_hip_quantized_gemm_f32": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint64] + [C.c_uint32] * 4),
     "yule_hip_quantized_gemm_noalloc": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint64] + [C.c_uint32] * 4),
+    "yule_hip_prompt_attn": (C.c_int, [C.c_void_p] * 5 + [C.c_uint64] + [C.c_uint32] * 6),
+    "yule_hip_prefix_attn": (C.c_int, [C.c_void_p] * 4 + [C.c_uint32, C.c_void_p, C.c_void_p, C.c_uint64, C.c_uint32,
+                                                          C.c_void_p] + [C.c_uint32] * 6),
+    "yule_hip_verify_drafts": (C.c_int, [C.c_void_p] * 3 + [C.c_uint64] * 5 + [C.c_uint32] * 3),
     "yule_hip_runner_create": (C.c_int, [C.c_void_p, C.c_void_p, C.POINTER(C.c_void_p)]),
     "yule_hip_runner_destroy": (C.c_int, [C.c_void_p]),
     "yule_hip_runner_reset": (C.c_int, [C.c_void_p]),
@@ -125,6 +129,14 @@ class BufferHandle:
     id: int
 
 
+class Rows(C.Structure):
+    """yule_rows: rows of a buffer `stride` elements apart, the first `offset` elements into it."""
+    _fields_ = [("buffer", C.c_uint64), ("offset", C.c_uint64), ("stride", C.c_uint64)]
+
+    def __init__(self, buffer, stride: int, offset: int = 0):
+        super().__init__(_h(buffer), offset, stride)
+
+
 @dataclass
 class DeviceInfo:
     """DeviceInfo, yule-gpu/src/lib.rs:137-143."""
@@ -160,6 +172,14 @@ def is_available() -> bool:
 
 def _h(x: BufferHandle | int) -> int:
     return x.id if isinstance(x, BufferHandle) else int(x)
+
+
+def _rows(x, width: int):
+    """A yule_rows argument: `Rows` as they are, a buffer as rows one after the other, None as null."""
+    return None if x is None else C.byref(x if isinstance(x, Rows) else Rows(x, width))
+
+
+NO_TOKEN = 0xFFFFFFFF   # YULE_NO_TOKEN
 
 
 class HipBackend:
@@ -315,6 +335,38 @@ class HipBackend:
         """quantized_gemm with its workspace in the library's static per-GPU array (no allocation)."""
         self._check(self._lib.yule_hip_quantized_gemm_noalloc(self._be, _h(weights), _h(x_bf16), _h(y), m, n_rows,
                                                               n_cols, int(dtype)))
+
+    def prompt_attn(self, q, k, v, out, offsets, n_seqs: int, n_rows: int, n_heads: int, n_kv_heads: int,
+                    head_dim: int, dtype: DType | int = DType.F32) -> None:
+        """Causal attention with grouped heads over packed prompts: sequence s is rows
+        offsets[s] .. offsets[s + 1] - 1.  q, k, v, out: buffers of rows one after the
+        other, or `Rows`."""
+        qd, kvd = n_heads * head_dim, n_kv_heads * head_dim
+        self._check(self._lib.yule_hip_prompt_attn(
+            self._be, _rows(q, qd), _rows(k, kvd), _rows(v, kvd), _rows(out, qd), _h(offsets), n_seqs, n_rows,
+            n_heads, n_kv_heads, head_dim, int(dtype)))
+
+    def prefix_attn(self, q, k_prefix, v_prefix, prefix_len: int, k_tail, v_tail, tail_lens, tail_cap: int, out,
+                    n_seqs: int, n_tokens: int, n_heads: int, n_kv_heads: int, head_dim: int,
+                    dtype: DType | int = DType.F32) -> None:
+        """Attention of each sequence's n_tokens newest tokens (rows s * n_tokens + i of q
+        and out) over a prefix that all sequences share and its own tail (rows s * tail_cap
+        .. of k_tail and v_tail, tail_lens[s] of them, the new tokens' last)."""
+        qd, kvd = n_heads * head_dim, n_kv_heads * head_dim
+        self._check(self._lib.yule_hip_prefix_attn(
+            self._be, _rows(q, qd), _rows(k_prefix, kvd), _rows(v_prefix, kvd), prefix_len, _rows(k_tail, kvd),
+            _rows(v_tail, kvd), _h(tail_lens), tail_cap, _rows(out, qd), n_seqs, n_tokens, n_heads, n_kv_heads,
+            head_dim, int(dtype)))
+
+    def verify_drafts(self, target, draft, draft_tokens, uniforms, draft_lens, accepted, tokens, n_seqs: int,
+                      n_draft: int, vocab: int) -> None:
+        """Drafts that stand against the target's probabilities, given uniform numbers:
+        accepted[s] of them, tokens[s] the kept drafts, the token after them, NO_TOKEN
+        behind it.  draft_lens None: n_draft each; n_draft 0: plain sampling (draft and
+        draft_tokens may be None)."""
+        self._check(self._lib.yule_hip_verify_drafts(
+            self._be, _rows(target, vocab), _rows(draft, vocab), _h(draft_tokens or 0), _h(uniforms),
+            _h(draft_lens or 0), _h(accepted), _h(tokens), n_seqs, n_draft, vocab))
 
     def time_qmv_ops(self, ops, iters: int, use_graph: bool = True) -> float:
         """Milliseconds (HIP events on the backend stream) for `iters` passes over

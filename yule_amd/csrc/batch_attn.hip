@@ -1,0 +1,719 @@
+// batch_attn.hip — attention of batches: packed prompts (yule_hip_prompt_attn)
+// and new tokens over a shared prefix and their own tails
+// (yule_hip_prefix_attn).  Grouped heads, f32, f16 and bf16.
+//
+// Both are the same walk.  The (query row, query head) pairs of one KV head are
+// its "slots", row by row with the group's heads side by side, so a key that is
+// read serves every head of the group.  A wave holds 32 slots and walks its keys
+// in subtiles of 32 with an online softmax:
+//   S^T = K Q^T      keys x slots, a lane holds 16 keys of one slot
+//   p = 2^(c S - m), m the running maximum of c S, c = log2(e) / sqrt(hd)
+//   O^T += V^T P^T   dims x slots; the lane's p are the operand as they lie
+// on the 32-row matrix instructions (operand row or column = lane % 32, k from h
+// = lane / 32; result column = lane % 32, row = 8 (i / 4) + 4 h + i % 4).  The
+// softmax reduces in the lane and across one swap of the halves.  A sum over k
+// does not mind the order of k, so 16-byte pieces of K and Q serve as operands
+// of any type, and P needs no rearranging: the keys of register i are taken from
+// V's rows instead.
+#include <cmath>
+#include <type_traits>
+
+#include "batch_plan.h"
+#include "internal.h"
+
+namespace yule {
+
+typedef int i4v __attribute__((ext_vector_type(4)));
+typedef float f4v __attribute__((ext_vector_type(4)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef _Float16 h8v __attribute__((ext_vector_type(8)));
+typedef __bf16 b8v __attribute__((ext_vector_type(8)));
+typedef short s4v __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) uint8_t *lds_b;
+typedef __attribute__((address_space(3))) s4v *lds_s4;
+
+// ---- matrix instructions by type: 16 bytes of each operand's row per lane
+template <typename T>
+__device__ __forceinline__ f16v mma16(i4v a, i4v b, f16v c) {
+    if constexpr (sizeof(T) == 4) {
+        const f4v x = __builtin_bit_cast(f4v, a), y = __builtin_bit_cast(f4v, b);
+#pragma unroll
+        for (int j = 0; j < 4; j++) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], y[j], c, 0, 0, 0);
+        return c;
+    } else if constexpr (__is_same(T, _Float16)) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8v, a), __builtin_bit_cast(h8v, b), c, 0, 0, 0);
+    } else {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8v, a), __builtin_bit_cast(b8v, b), c, 0, 0, 0);
+    }
+}
+
+// eight probabilities as an operand, rounded to the type (2^-9 or 2^-12 of each
+// value at most: below the rounding of V itself; the weight's sum keeps f32)
+template <typename T>
+__device__ __forceinline__ i4v pack8(const f16v &s, int at) {
+    if constexpr (__is_same(T, _Float16)) {
+        h8v r;
+#pragma unroll
+        for (int j = 0; j < 8; j++) r[j] = (_Float16)s[at + j];
+        return __builtin_bit_cast(i4v, r);
+    } else {
+        b8v r;
+#pragma unroll
+        for (int j = 0; j < 8; j++) r[j] = (__bf16)s[at + j];
+        return __builtin_bit_cast(i4v, r);
+    }
+}
+
+// some element of 16 bytes is infinite or NaN
+template <typename T>
+__device__ __forceinline__ bool not_finite(i4v x) {
+    constexpr uint32_t E = sizeof(T) == 4 ? 0x7f800000u : __is_same(T, _Float16) ? 0x7c00u : 0x7f80u;
+    bool bad = false;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+        const uint32_t w = (uint32_t)x[j];
+        bad |= (w & E) == E;
+        if constexpr (sizeof(T) == 2) bad |= (w & (E << 16)) == (E << 16);
+    }
+    return bad;
+}
+
+// ---- a subtile in LDS: 32 rows of D elements as C 16-byte chunks, chunk c of
+// row r at chunk c ^ swizzle(r) of its row.  P rows fill the 256 bytes of all
+// banks, and the XOR walks the G chunks that a power of two divides off C: 16
+// rows of one chunk (K operands), and 8 rows of two chunks (step 2: V operands),
+// lie in different banks.
+template <uint32_t C, uint32_t STEP>
+__device__ __forceinline__ uint32_t swizzle(uint32_t r) {
+    constexpr uint32_t G = C % 16 == 0 ? 16 : C % 8 == 0 ? 8 : C % 4 == 0 ? 4 : 2, P = 16 / G;
+    return (STEP * (r / P)) % G;
+}
+
+// outside the compiler's memory model, its waits included: every wait for it is
+// explicit, and so is the wait state after a scalar write of M0
+__device__ __forceinline__ void copy_to_lds(const uint8_t *base, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base),
+                 "s"(__builtin_amdgcn_readfirstlane(lds))
+                 : "m0", "memory");
+}
+template <uint32_t N>
+__device__ __forceinline__ void wait_copies() {   // until at most N are in flight
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// x as the compiler knows nothing about it: what is computed from it is computed
+// there, and not kept in registers over the loop (operand and copy addresses: a
+// few integer operations each, beside hundreds of registers)
+__device__ __forceinline__ uint32_t opaque(uint32_t x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+
+// rows of a cache or activation: address of row 0 of one head, bytes between rows
+struct Rows {
+    const uint8_t *p;
+    uint32_t stride;
+};
+
+// ---- one wave: 32 slots over keys key0, key0 + step, .. < k1 (subtiles of 32)
+template <typename T, uint32_t D>
+struct WaveAttn {
+    static constexpr uint32_t SZ = sizeof(T), RB = D * SZ, C = RB / 16, SUB = 32 * RB;
+    static constexpr uint32_t NL = SUB / 1024, NS = RB / 32, DT = D / 32;
+    i4v q[NS];    // bytes 32 s + 16 h .. of this lane's slot's query
+    f16v o[DT];   // O^T, unnormalised: dim 32 t + 8 (i / 4) + 4 h + i % 4
+    float m, l;   // running maximum of c S; this lane's share of the weight's sum
+
+    __device__ __forceinline__ void init(const uint8_t *qrow, uint32_t hb, uint32_t h) {
+#pragma unroll
+        for (uint32_t s = 0; s < NS; s++) {
+            const uint32_t at = 32 * s + 16 * h;
+            q[s] = i4v{0, 0, 0, 0};
+            if (at < hb) q[s] = *reinterpret_cast<const i4v *>(qrow + at);
+        }
+#pragma unroll
+        for (uint32_t t = 0; t < DT; t++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[t][i] = 0.f;
+        m = -INFINITY;
+        l = 0.f;
+    }
+
+    // the subtile's scores into probabilities, sums rescaled where a maximum moved
+    __device__ __forceinline__ void softmax(f16v &s, float c) {
+        float cm = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; i++) cm = fmaxf(cm, s[i]);
+        cm = fmaxf(cm, __shfl_xor(cm, 32, 64)) * c;
+        if (__ballot(cm > m)) {
+            const float mn = fmaxf(m, cm);
+            // (m = -inf: nothing was added yet, and the factor multiplies zeros)
+            const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (uint32_t t = 0; t < DT; t++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[t][i] *= alpha;
+        }
+        const float mb = m == -INFINITY ? 0.f : m;   // nothing seen yet: weights of 0
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -mb));
+            l += s[i];
+        }
+    }
+
+    // O^T += V^T P^T with V's subtile at v
+    __device__ __forceinline__ void values(const f16v &s, const uint8_t *v, uint32_t tid) {
+        const uint32_t lane = opaque(tid) & 63u, h = lane >> 5;
+        if constexpr (SZ == 4) {
+            const uint32_t d = lane & 31u;
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const uint32_t r = 8 * (i / 4) + 4 * h + i % 4;
+#pragma unroll
+                for (uint32_t t = 0; t < DT; t++) {
+                    const float a = *reinterpret_cast<const float *>(
+                        v + r * RB + (((8 * t + (d >> 2)) ^ swizzle<C, 2>(r)) << 4) + 4 * (d & 3u));
+                    o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, s[i], o[t], 0, 0, 0);
+                }
+            }
+        } else {
+            // the transposing read gives lane l of 16 column l of the four rows that lanes 4 r .. 4 r + 3 point
+            // to: here the dims of V^T's rows from four keys
+            const uint32_t e = lane & 15u, g = lane >> 4;
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const i4v p = pack8<T>(s, 8 * k);
+                const uint32_t r0 = 16 * k + 4 * h + (e >> 2), r1 = r0 + 8;
+#pragma unroll
+                for (uint32_t t = 0; t < DT; t++) {
+                    const uint32_t ch = 4 * t + 2 * (g & 1u) + ((e & 3u) >> 1), sub = 8 * (e & 1u);
+                    const s4v a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (lds_s4)(lds_b)(v + r0 * RB + ((ch ^ swizzle<C, 2>(r0)) << 4) + sub));
+                    const s4v a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (lds_s4)(lds_b)(v + r1 * RB + ((ch ^ swizzle<C, 2>(r1)) << 4) + sub));
+                    const auto a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
+                    o[t] = mma16<T>(__builtin_bit_cast(i4v, a), p, o[t]);
+                }
+            }
+        }
+    }
+
+    // The same, key by key, for a subtile some of whose keys are hidden from some
+    // slots and whose V holds an infinity or a NaN: 0 times that is not 0, so
+    // hidden keys have to be left out, not weighted with 0.  (key0: the
+    // subtile's first key; the slot sees keys below lim.)
+    __device__ __forceinline__ void values_seen(const f16v &s, const uint8_t *v, uint32_t tid, uint32_t key0,
+                                                uint32_t lim) {
+        const uint32_t lane = opaque(tid) & 63u, h = lane >> 5;
+#pragma unroll 1
+        for (uint32_t k = 0; k < 32; k++) {
+            const uint32_t at = 4 * (k >> 3) + (k & 3u);
+            float p = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; i++) p = at == (uint32_t)i ? s[i] : p;
+            p = __shfl(p, 32 * ((k >> 2) & 1u) + (lane & 31u), 64);
+            if (key0 + k >= lim) continue;
+#pragma unroll
+            for (uint32_t t = 0; t < DT; t++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    if (i % 4 == 0) __builtin_amdgcn_sched_barrier(0);   // (few values in registers at a time)
+                    const uint32_t d = 32 * t + 8 * (i / 4) + 4 * h + i % 4;
+                    const uint8_t *x = v + k * RB + (((d * SZ / 16) ^ swizzle<C, 2>(k)) << 4) + d * SZ % 16;
+                    o[t][i] = fmaf(p, (float)*reinterpret_cast<const T *>(x), o[t][i]);
+                }
+        }
+    }
+
+    // Keys key, key + step, .. < k1 in subtiles of 32 (lds: this wave's K subtile
+    // and V subtile).  A slot sees keys below lim; every slot sees those below
+    // lim_all.  The next K subtile is on its way while this one's softmax and
+    // product with V run, the next V subtile during the next scores: copies
+    // complete in order, so "at most NL in flight" says that the older of the
+    // two has landed.
+    __device__ __forceinline__ void walk(const Rows &K, const Rows &V, uint32_t hb, uint32_t key, uint32_t step,
+                                         uint32_t k1, uint32_t lim, uint32_t lim_all, uint8_t *lds, uint32_t lane,
+                                         float c) {
+        const uint32_t h = lane >> 5;
+        const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)reinterpret_cast<uintptr_t>((lds_b)lds));
+        uint8_t *const vt = lds + SUB;
+        if (hb < RB) {   // chunks past the head stay zero: copies leave them out
+#pragma unroll
+            for (uint32_t i = 0; i < 2 * NL; i++) *reinterpret_cast<i4v *>(lds + 1024 * i + 16 * lane) = i4v{0, 0, 0, 0};
+            wait_lds();
+        }
+        // Lane's part of copy i: LDS chunk 64 i + lane of the subtile.  Rows past
+        // the last key repeat it (hidden, and the number of copies stays).
+        auto copy = [&](const Rows &R, auto is_v, uint32_t at) {
+            constexpr uint32_t STEP = decltype(is_v)::value ? 2 : 1;
+            const uint64_t row = reinterpret_cast<uint64_t>(R.p) + (uint64_t)at * R.stride;
+            const uint8_t *base = reinterpret_cast<const uint8_t *>(
+                (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(row >> 32)) << 32 |
+                (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)row));
+            const uint32_t last = k1 - at - 1u, ln = opaque(lane) & 63u;
+#pragma unroll
+            for (uint32_t i = 0; i < NL; i++) {
+                const uint32_t L = 64 * i + ln, r = L / C, ch = (L % C) ^ swizzle<C, STEP>(r);
+                if (16 * ch < hb)
+                    copy_to_lds(base, (r < last ? r : last) * R.stride + 16 * ch,
+                                lds0 + (decltype(is_v)::value ? SUB : 0u) + 1024 * i);
+            }
+        };
+        using No = std::false_type;
+        using Yes = std::true_type;
+        if (key < k1) {
+            copy(K, No{}, key);
+            copy(V, Yes{}, key);
+        }
+        for (; key < k1; key += step) {
+            const bool more = key + step < k1;
+            wait_copies<NL>();   // K is there
+            f16v s;
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[i] = 0.f;
+            {
+                const uint32_t ln = opaque(lane) & 63u, r = ln & 31u, hh = ln >> 5;
+#pragma unroll
+                for (uint32_t st = 0; st < NS; st++) {
+                    const i4v a = *reinterpret_cast<const i4v *>(lds + r * RB + (((2 * st + hh) ^ swizzle<C, 1>(r)) << 4));
+                    s = mma16<T>(a, q[st], s);
+                }
+            }
+            wait_lds();
+            if (more) copy(K, No{}, key + step);
+            const bool masked = key + 32 > lim_all;
+            if (masked) {
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+                    if (key + 8 * (i / 4) + 4 * h + i % 4 >= lim) s[i] = -INFINITY;
+            }
+            softmax(s, c);
+            if (more) wait_copies<NL>();   // V is there
+            else wait_copies<0>();
+            bool odd = false;
+            if (masked) {
+#pragma unroll
+                for (uint32_t i = 0; i < NL; i++)
+                    odd |= not_finite<T>(*reinterpret_cast<const i4v *>(vt + 1024 * i + 16 * lane));
+                odd = __ballot(odd) != 0;
+            }
+            if (odd) values_seen(s, vt, lane, key, lim);
+            else values(s, vt, lane);
+            wait_lds();
+            if (more) copy(V, Yes{}, key + step);
+        }
+    }
+};
+
+// ---- a workgroup: NW waves share 32 slots and take the keys' subtiles in turn
+template <typename T, uint32_t D>
+struct BlockAttn {
+    using W = WaveAttn<T, D>;
+    // waves whose subtiles fit the LDS (f32 heads of 256 dims: 64 KB a wave)
+    static constexpr uint32_t NW = 2 * W::SUB * 4 <= 131072 ? 4 : 2;
+    // waves a SIMD that the LDS has room for: the registers are to allow them too
+    static constexpr uint32_t WAVES = 2 * W::SUB * 4 <= 65536 ? 2 : 1;
+    struct Shared {
+        __align__(1024) uint8_t tiles[NW][2 * W::SUB];
+        float m[NW][32], l[NW][32];
+    };
+
+    // out(slot of 32, dim, four sums, maximum, weight): joined over the waves
+    template <typename OUT>
+    __device__ __forceinline__ static void run(Shared &sh, const uint8_t *qrow, const Rows &K, const Rows &V,
+                                               uint32_t hb, uint32_t k0, uint32_t k1, uint32_t lim, uint32_t lim_all,
+                                               float c, OUT out) {
+        const uint32_t tid = threadIdx.x, lane = tid & 63u, h = lane >> 5, r32 = lane & 31u;
+        const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        W w;
+        w.init(qrow, hb, h);
+        w.walk(K, V, hb, k0 + 32 * wave, 32 * NW, k1, lim, lim_all, sh.tiles[wave], lane, c);
+        const float l = w.l + __shfl_xor(w.l, 32, 64);
+        if (h == 0) {
+            sh.m[wave][r32] = w.m;
+            sh.l[wave][r32] = l;
+        }
+        // the wave's subtiles make room for its sums, f32 [32][D], chunks XORed with the row (the writes of
+        // eight lanes lie in different banks)
+        uint8_t *const ob = sh.tiles[wave];
+#pragma unroll
+        for (uint32_t t = 0; t < W::DT; t++)
+#pragma unroll
+            for (uint32_t a = 0; a < 4; a++)
+                *reinterpret_cast<f4v *>(ob + r32 * D * 4 + (((8 * t + 2 * a + h) ^ (r32 & 7u)) << 4)) =
+                    f4v{w.o[t][4 * a], w.o[t][4 * a + 1], w.o[t][4 * a + 2], w.o[t][4 * a + 3]};
+        __syncthreads();
+        for (uint32_t i = tid; i < 32 * (D / 4); i += 64 * NW) {
+            const uint32_t r = i / (D / 4), ch = i % (D / 4);
+            float M = sh.m[0][r];
+#pragma unroll
+            for (uint32_t x = 1; x < NW; x++) M = fmaxf(M, sh.m[x][r]);
+            float L = 0.f;
+            f4v acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (uint32_t x = 0; x < NW; x++) {
+                // (a wave that saw no key of the slot has zeros, and m = -inf)
+                const float f = sh.m[x][r] == -INFINITY ? (M == -INFINITY ? 1.f : 0.f) : __builtin_amdgcn_exp2f(sh.m[x][r] - M);
+                const f4v o = *reinterpret_cast<const f4v *>(sh.tiles[x] + r * D * 4 + ((ch ^ (r & 7u)) << 4));
+                L += f * sh.l[x][r];
+                acc += f * o;
+            }
+            out(r, 4 * ch, acc, M, L);
+        }
+    }
+};
+
+// four results of a row, rounded once to its type
+template <typename T>
+__device__ __forceinline__ void store4(uint8_t *row, uint32_t d, f4v x) {
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<f4v *>(row + 4 * d) = x;
+    } else {
+        typedef T t4 __attribute__((ext_vector_type(4)));
+        *reinterpret_cast<t4 *>(row + 2 * d) = t4{(T)x[0], (T)x[1], (T)x[2], (T)x[3]};
+    }
+}
+
+struct HeadShape {
+    uint32_t group, n_kv, hd;   // query heads per KV head, KV heads, dims
+    float c;                    // log2(e) / sqrt(hd)
+};
+
+// ---- packed prompts
+struct PromptArgs {
+    const uint8_t *q, *k, *v;
+    uint8_t *out;
+    uint32_t qs, ks, vs, os;    // bytes between rows
+    const uint32_t *off;
+    uint32_t n_seqs, n_rows;
+    HeadShape s;
+};
+
+// Query tile y of the batch: its sequence's first row and length, and the tile
+// inside it (tiles of a sequence from the last, with the most keys, to the
+// first).  Offsets are the caller's data on the device: rows are clamped to the
+// buffers'.  False past the last tile.
+__device__ __forceinline__ bool find_tile(const uint32_t *off, uint32_t n_seqs, uint32_t n_rows, uint32_t group,
+                                          uint32_t y, uint32_t lane, uint32_t *row0, uint32_t *len, uint32_t *tile) {
+    uint32_t before = 0;
+    for (uint32_t s0 = 0; s0 < n_seqs; s0 += 64) {
+        const uint32_t s = s0 + lane;
+        uint32_t b = 0, e = 0;
+        if (s < n_seqs) {
+            b = off[s];
+            e = off[s + 1];
+            b = b < n_rows ? b : n_rows;
+            e = e < n_rows ? e : n_rows;
+            e = e > b ? e : b;
+        }
+        const uint32_t mine = ((e - b) * group + kAttnTileRows - 1) / kAttnTileRows;
+        uint32_t sum = mine;
+#pragma unroll
+        for (uint32_t d = 1; d < 64; d *= 2) {
+            const uint32_t x = __shfl_up(sum, d, 64);
+            if (lane >= d) sum += x;
+        }
+        const uint64_t here = __ballot(before + sum > y);
+        if (here) {
+            const int at = __builtin_ctzll(here);
+            *row0 = __builtin_amdgcn_readlane(b, at);
+            *len = __builtin_amdgcn_readlane(e - b, at);
+            *tile = before + __builtin_amdgcn_readlane(sum, at) - 1u - y;
+            return true;
+        }
+        before += __builtin_amdgcn_readlane(sum, 63);
+    }
+    return false;
+}
+
+template <typename T, uint32_t D>
+__global__ __launch_bounds__((64 * BlockAttn<T, D>::NW))
+    __attribute__((amdgpu_waves_per_eu(BlockAttn<T, D>::WAVES))) void prompt_attn_kernel(PromptArgs a) {
+    using B = BlockAttn<T, D>;
+    __shared__ typename B::Shared sh;
+    const uint32_t kvh = blockIdx.x % a.s.n_kv, lane = threadIdx.x & 63u;
+    uint32_t row0, len, tile;
+    if (!find_tile(a.off, a.n_seqs, a.n_rows, a.s.group, blockIdx.x / a.s.n_kv, lane, &row0, &len, &tile)) return;
+    const uint32_t slots = len * a.s.group, slot0 = tile * kAttnTileRows, hb = a.s.hd * sizeof(T);
+    const uint32_t last = (slot0 + kAttnTileRows < slots ? slot0 + kAttnTileRows : slots) - 1u;
+    auto at = [&](uint32_t slot, uint32_t stride) {   // the slot's bytes in q or out
+        const uint32_t r = slot / a.s.group;
+        return (size_t)(row0 + r) * stride + (size_t)(kvh * a.s.group + (slot - r * a.s.group)) * hb;
+    };
+    const uint32_t mine = slot0 + (lane & 31u) < last ? slot0 + (lane & 31u) : last;
+    const Rows K = {a.k + (size_t)row0 * a.ks + (size_t)kvh * hb, a.ks}, V = {a.v + (size_t)row0 * a.vs + (size_t)kvh * hb, a.vs};
+    B::run(sh, a.q + at(mine, a.qs), K, V, hb, 0, last / a.s.group + 1u, mine / a.s.group + 1u, slot0 / a.s.group + 1u,
+           a.s.c, [&](uint32_t r, uint32_t d, f4v o, float, float L) {
+               if (slot0 + r <= last && d < a.s.hd) store4<T>(a.out + at(slot0 + r, a.os), d, o * (L == 0.f ? 0.f : 1.0f / L));
+           });
+}
+
+// ---- new tokens over a shared prefix and their own tails
+struct PrefixArgs {
+    const uint8_t *q, *kp, *vp, *kt, *vt;
+    uint32_t qs, kps, vps, kts, vts;
+    const uint32_t *lens;
+    uint32_t prefix, cap, n_seqs, n_tokens;
+    uint32_t p_chunk, n_p, p_tiles, t_chunk, n_t, t_tiles, p_jobs;
+    float2 *ml;   // [chunk][row][head]
+    float *o;     // [chunk][row][head][hd]
+    HeadShape s;
+};
+
+template <typename T, uint32_t D>
+__global__ __launch_bounds__((64 * BlockAttn<T, D>::NW))
+    __attribute__((amdgpu_waves_per_eu(BlockAttn<T, D>::WAVES))) void prefix_attn_kernel(PrefixArgs a) {
+    using B = BlockAttn<T, D>;
+    __shared__ typename B::Shared sh;
+    const uint32_t lane = threadIdx.x & 63u, hb = a.s.hd * sizeof(T), g = a.s.group, n_heads = g * a.s.n_kv;
+    uint32_t job = blockIdx.x, row0, slots, tile, chunk, k0, k1, lim, lim_all;
+    const uint32_t kvh = job % a.s.n_kv;
+    Rows K, V;
+    uint32_t last, slot0, mine;
+    auto place = [&]() {
+        slot0 = tile * kAttnTileRows;
+        last = (slot0 + kAttnTileRows < slots ? slot0 + kAttnTileRows : slots) - 1u;
+        mine = slot0 + (lane & 31u) < last ? slot0 + (lane & 31u) : last;
+    };
+    if (job < a.p_jobs) {
+        job /= a.s.n_kv;
+        tile = job % a.p_tiles;
+        chunk = job / a.p_tiles;
+        row0 = 0;
+        slots = a.n_seqs * a.n_tokens * g;
+        place();
+        k0 = chunk * a.p_chunk;
+        k1 = a.prefix - k0 < a.p_chunk ? a.prefix : k0 + a.p_chunk;
+        lim = lim_all = k1;
+        K = {a.kp + (size_t)kvh * hb, a.kps};
+        V = {a.vp + (size_t)kvh * hb, a.vps};
+    } else {
+        job = (job - a.p_jobs) / a.s.n_kv;
+        tile = job % a.t_tiles;
+        job /= a.t_tiles;
+        const uint32_t seq = job % a.n_seqs, len = a.lens[seq] < a.cap ? a.lens[seq] : a.cap;
+        chunk = job / a.n_seqs;
+        row0 = seq * a.n_tokens;
+        slots = a.n_tokens * g;
+        place();
+        // token i sees rows below len - n_tokens + 1 + i of the tail
+        auto sees = [&](uint32_t slot) {
+            const uint32_t n = len + 1u + slot / g;
+            return n > a.n_tokens ? n - a.n_tokens : 0u;
+        };
+        k0 = chunk * a.t_chunk;
+        k1 = sees(last) < k0 + a.t_chunk ? sees(last) : k0 + a.t_chunk;
+        lim = sees(mine) < k1 ? sees(mine) : k1;
+        lim_all = sees(slot0);
+        K = {a.kt + (size_t)seq * a.cap * a.kts + (size_t)kvh * hb, a.kts};
+        V = {a.vt + (size_t)seq * a.cap * a.vts + (size_t)kvh * hb, a.vts};
+        chunk += a.n_p;
+    }
+    auto pair = [&](uint32_t slot) {   // (row, head) of the slot
+        const uint32_t r = slot / g;
+        return (size_t)(row0 + r) * n_heads + kvh * g + (slot - r * g);
+    };
+    const size_t part = (size_t)chunk * a.n_seqs * a.n_tokens * n_heads;
+    if (k0 >= k1) {   // nothing of the tail in this chunk
+        if (threadIdx.x < 32 && slot0 + threadIdx.x <= last) a.ml[part + pair(slot0 + threadIdx.x)] = make_float2(-INFINITY, 0.f);
+        return;
+    }
+    const uint32_t r = mine / g;
+    B::run(sh, a.q + (size_t)(row0 + r) * a.qs + (size_t)(kvh * g + (mine - r * g)) * hb, K, V, hb, k0, k1, lim, lim_all, a.s.c,
+           [&](uint32_t i, uint32_t d, f4v o, float M, float L) {
+               if (slot0 + i > last || d >= a.s.hd) return;
+               const size_t at = part + pair(slot0 + i);
+               if (d == 0) a.ml[at] = make_float2(M, L);
+               *reinterpret_cast<f4v *>(a.o + at * a.s.hd + d) = o;
+           });
+}
+
+// out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c over a row's chunks, a wave
+// per (row, head).  A row that saw no key has l = 0 everywhere and gives zeros.
+template <typename T>
+__global__ __launch_bounds__(256) void prefix_join_kernel(const float2 *__restrict__ ml, const float *__restrict__ o,
+                                                          uint8_t *__restrict__ out, uint32_t os, uint32_t rows,
+                                                          uint32_t n_heads, uint32_t hd, uint32_t parts) {
+    const uint32_t at = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63u;
+    if (at >= rows) return;
+    float M = -INFINITY;
+    for (uint32_t p = lane; p < parts; p += 64) M = fmaxf(M, ml[(size_t)p * rows + at].x);
+#pragma unroll
+    for (uint32_t d = 32; d; d /= 2) M = fmaxf(M, __shfl_xor(M, d, 64));
+    float L = 0.f;
+    f4v acc = {0.f, 0.f, 0.f, 0.f};
+    for (uint32_t p = 0; p < parts; p++) {
+        const float2 x = ml[(size_t)p * rows + at];
+        if (x.x == -INFINITY && x.y == 0.f) continue;   // no key of this chunk: its sums were not written
+        const float f = __builtin_amdgcn_exp2f(x.x - M);
+        L += f * x.y;
+        if (4 * lane < hd) acc += f * *reinterpret_cast<const f4v *>(o + ((size_t)p * rows + at) * hd + 4 * lane);
+    }
+    const float inv = L == 0.f ? 0.f : 1.0f / L;
+    const uint32_t row = at / n_heads;
+    if (4 * lane < hd)
+        store4<T>(out + (size_t)row * os + (size_t)(at - row * n_heads) * hd * sizeof(T), 4 * lane, acc * inv);
+}
+
+// f(element type, padded head size)
+template <typename F>
+static void by_shape(uint32_t dtype, uint32_t hd, F f) {
+    auto dims = [&](auto t) {
+        switch (attn_padded_dim(hd)) {
+        case 64: f(t, std::integral_constant<uint32_t, 64>{}); break;
+        case 96: f(t, std::integral_constant<uint32_t, 96>{}); break;
+        case 128: f(t, std::integral_constant<uint32_t, 128>{}); break;
+        default: f(t, std::integral_constant<uint32_t, 256>{}); break;
+        }
+    };
+    if (dtype == YULE_DTYPE_F32) dims(float{});
+    else if (dtype == YULE_DTYPE_F16) dims((_Float16)0);
+    else dims((__bf16)0);
+}
+
+static HeadShape head_shape(uint32_t n_heads, uint32_t n_kv, uint32_t hd) {
+    return {n_heads / n_kv, n_kv, hd, (float)(1.44269504088896340736 / sqrt((double)hd))};
+}
+
+static int launch_prompt(hipStream_t s, const PromptArgs &a, uint32_t dtype, uint64_t workgroups) {
+    by_shape(dtype, a.s.hd, [&](auto t, auto d) {
+        using T = decltype(t);
+        constexpr uint32_t D = decltype(d)::value;
+        hipLaunchKernelGGL((prompt_attn_kernel<T, D>), dim3((uint32_t)workgroups), dim3(64 * BlockAttn<T, D>::NW), 0, s, a);
+    });
+    return check_launch("prompt_attn");
+}
+
+static int launch_prefix(hipStream_t s, const PrefixArgs &a, uint32_t dtype, uint64_t workgroups) {
+    by_shape(dtype, a.s.hd, [&](auto t, auto d) {
+        using T = decltype(t);
+        constexpr uint32_t D = decltype(d)::value;
+        hipLaunchKernelGGL((prefix_attn_kernel<T, D>), dim3((uint32_t)workgroups), dim3(64 * BlockAttn<T, D>::NW), 0, s, a);
+    });
+    return check_launch("prefix_attn");
+}
+
+static int launch_join(hipStream_t s, const PrefixArgs &a, uint8_t *out, uint32_t os, uint32_t dtype) {
+    const uint32_t n_heads = a.s.group * a.s.n_kv, rows = a.n_seqs * a.n_tokens * n_heads;
+    auto go = [&](auto t) {
+        hipLaunchKernelGGL((prefix_join_kernel<decltype(t)>), dim3((rows + 3) / 4), dim3(256), 0, s, a.ml, a.o, out, os,
+                           rows, n_heads, a.s.hd, a.n_p + a.n_t);
+    };
+    if (dtype == YULE_DTYPE_F32) go(float{});
+    else if (dtype == YULE_DTYPE_F16) go((_Float16)0);
+    else go((__bf16)0);
+    return check_launch("prefix_attn (join)");
+}
+
+// ---- C entries
+namespace {
+
+struct Checked {
+    uint8_t *p;
+    uint32_t stride;   // bytes
+};
+
+int rows_arg(yule_hip_backend *be, const yule_rows *r, uint64_t n_rows, uint64_t width, uint32_t elem, const char *what,
+             Checked *out) {
+    void *p;
+    int rc = rows_ptr(be, r, n_rows, width, elem, 16, what, &p);
+    if (rc) return rc;
+    out->p = static_cast<uint8_t *>(p);
+    out->stride = n_rows > 1 ? (uint32_t)(r->stride * elem) : 0u;   // (one row or none: any stride is given)
+    return YULE_OK;
+}
+
+}  // namespace
+}  // namespace yule
+
+using namespace yule;
+
+extern "C" {
+
+int yule_hip_prompt_attn(yule_hip_backend *be, const yule_rows *q, const yule_rows *k, const yule_rows *v,
+                         const yule_rows *out, yule_buffer offsets, uint32_t n_seqs, uint32_t n_rows, uint32_t n_heads,
+                         uint32_t n_kv_heads, uint32_t head_dim, uint32_t dtype) {
+    return guarded("prompt_attn", be, [&]() -> int {
+        const uint32_t elem = attn_elem_bytes(dtype);
+        if (!elem) return set_error(YULE_ERR_UNSUPPORTED, "prompt_attn: dtype " + std::to_string(dtype) + " not supported");
+        if (const char *bad = check_heads(n_heads, n_kv_heads, head_dim))
+            return set_error(YULE_ERR_INVALID, std::string("prompt_attn: ") + bad);
+        const uint64_t qd = (uint64_t)n_heads * head_dim, kvd = (uint64_t)n_kv_heads * head_dim;
+        Checked cq, ck, cv, co;
+        void *off;
+        int rc;
+        if ((rc = rows_arg(be, q, n_rows, qd, elem, "prompt_attn (q)", &cq)) ||
+            (rc = rows_arg(be, k, n_rows, kvd, elem, "prompt_attn (k)", &ck)) ||
+            (rc = rows_arg(be, v, n_rows, kvd, elem, "prompt_attn (v)", &cv)) ||
+            (rc = rows_arg(be, out, n_rows, qd, elem, "prompt_attn (out)", &co)) ||
+            (rc = get_buffer(be, offsets, ((size_t)n_seqs + 1) * 4, &off, "prompt_attn (offsets)")))
+            return rc;
+        if (out->buffer == q->buffer || out->buffer == k->buffer || out->buffer == v->buffer || out->buffer == offsets)
+            return set_error(YULE_ERR_INVALID, "prompt_attn: an input and the output alias");
+        if (!n_seqs || !n_rows) return YULE_OK;
+        // tiles of all sequences: each has at most one that is not full
+        const uint64_t group = n_heads / n_kv_heads, tiles = n_rows * group / kAttnTileRows + n_seqs;
+        if ((uint64_t)n_rows * group >= (uint64_t)1 << 31 || tiles * n_kv_heads > kMaxWorkgroups)
+            return set_error(YULE_ERR_INVALID, "prompt_attn: too many rows for one call");
+        const PromptArgs a = {cq.p, ck.p, cv.p, co.p, cq.stride, ck.stride, cv.stride, co.stride,
+                              static_cast<const uint32_t *>(off), n_seqs, n_rows, head_shape(n_heads, n_kv_heads, head_dim)};
+        return launch_prompt(be->stream, a, dtype, tiles * n_kv_heads);
+    });
+}
+
+int yule_hip_prefix_attn(yule_hip_backend *be, const yule_rows *q, const yule_rows *k_prefix, const yule_rows *v_prefix,
+                         uint32_t prefix_len, const yule_rows *k_tail, const yule_rows *v_tail, yule_buffer tail_lens,
+                         uint32_t tail_cap, const yule_rows *out, uint32_t n_seqs, uint32_t n_tokens, uint32_t n_heads,
+                         uint32_t n_kv_heads, uint32_t head_dim, uint32_t dtype) {
+    return guarded("prefix_attn", be, [&]() -> int {
+        const uint32_t elem = attn_elem_bytes(dtype);
+        if (!elem) return set_error(YULE_ERR_UNSUPPORTED, "prefix_attn: dtype " + std::to_string(dtype) + " not supported");
+        if (const char *bad = check_heads(n_heads, n_kv_heads, head_dim))
+            return set_error(YULE_ERR_INVALID, std::string("prefix_attn: ") + bad);
+        if (!n_tokens || n_tokens > 64) return set_error(YULE_ERR_INVALID, "prefix_attn: n_tokens must be 1..64");
+        if (prefix_len > kMaxKeys || tail_cap > kMaxKeys)
+            return set_error(YULE_ERR_INVALID, "prefix_attn: more than 2^30 keys");
+        const uint64_t qd = (uint64_t)n_heads * head_dim, kvd = (uint64_t)n_kv_heads * head_dim;
+        const uint64_t rows = (uint64_t)n_seqs * n_tokens, tails = (uint64_t)n_seqs * tail_cap;
+        Checked cq, ckp = {}, cvp = {}, ckt = {}, cvt = {}, co;
+        void *lens;
+        int rc;
+        if ((rc = rows_arg(be, q, rows, qd, elem, "prefix_attn (q)", &cq)) ||
+            (prefix_len && ((rc = rows_arg(be, k_prefix, prefix_len, kvd, elem, "prefix_attn (k_prefix)", &ckp)) ||
+                            (rc = rows_arg(be, v_prefix, prefix_len, kvd, elem, "prefix_attn (v_prefix)", &cvp)))) ||
+            (tail_cap && ((rc = rows_arg(be, k_tail, tails, kvd, elem, "prefix_attn (k_tail)", &ckt)) ||
+                          (rc = rows_arg(be, v_tail, tails, kvd, elem, "prefix_attn (v_tail)", &cvt)))) ||
+            (rc = rows_arg(be, out, rows, qd, elem, "prefix_attn (out)", &co)) ||
+            (rc = get_buffer(be, tail_lens, (size_t)n_seqs * 4, &lens, "prefix_attn (tail_lens)")))
+            return rc;
+        if (out->buffer == q->buffer || out->buffer == tail_lens ||
+            (prefix_len && (out->buffer == k_prefix->buffer || out->buffer == v_prefix->buffer)) ||
+            (tail_cap && (out->buffer == k_tail->buffer || out->buffer == v_tail->buffer)))
+            return set_error(YULE_ERR_INVALID, "prefix_attn: an input and the output alias");
+        if (!n_seqs) return YULE_OK;
+        const PrefixPlan p = prefix_plan(prefix_len, tail_cap, n_seqs, n_tokens, n_heads, n_kv_heads, head_dim,
+                                         (uint32_t)be->props.multiProcessorCount);
+        if (p.rows >= (uint64_t)1 << 25 || p.p_jobs + p.t_jobs > kMaxWorkgroups)
+            return set_error(YULE_ERR_INVALID, "prefix_attn: too many rows for one call");
+        ScratchLease ws;   // held until both launches are enqueued
+        if ((rc = get_scratch(be, p.bytes(), &ws))) return rc;
+        PrefixArgs a = {};
+        a.q = cq.p, a.kp = ckp.p, a.vp = cvp.p, a.kt = ckt.p, a.vt = cvt.p;
+        a.qs = cq.stride, a.kps = ckp.stride, a.vps = cvp.stride, a.kts = ckt.stride, a.vts = cvt.stride;
+        a.lens = static_cast<const uint32_t *>(lens);
+        a.prefix = prefix_len, a.cap = tail_cap, a.n_seqs = n_seqs, a.n_tokens = n_tokens;
+        a.p_chunk = p.p_chunk, a.n_p = p.n_p, a.p_tiles = p.p_tiles;
+        a.t_chunk = p.t_chunk, a.n_t = p.n_t, a.t_tiles = p.t_tiles, a.p_jobs = (uint32_t)p.p_jobs;
+        a.ml = static_cast<float2 *>(ws.ptr);
+        a.o = reinterpret_cast<float *>(static_cast<uint8_t *>(ws.ptr) + p.ml_bytes);
+        a.s = head_shape(n_heads, n_kv_heads, head_dim);
+        if (p.p_jobs + p.t_jobs && (rc = launch_prefix(be->stream, a, dtype, p.p_jobs + p.t_jobs))) return rc;
+        return launch_join(be->stream, a, co.p, co.stride, dtype);
+    });
+}
+
+}  // extern "C"

@@ -1,0 +1,103 @@
+// batch_plan.h — what the batched serving operators decide on the host: the
+// checks of their arguments, how work is split, and where results that are
+// joined later lie in the workspace.  Plain C++ (no HIP), so that a program
+// without a GPU can check it.
+#pragma once
+
+#include <cstddef>
+#include <cstdint>
+#include <cstdio>
+
+#include "../../include/yule_hip.h"
+
+namespace yule {
+
+// bytes of one element of an attention type; 0: not one
+inline uint32_t attn_elem_bytes(uint32_t dtype) {
+    return dtype == YULE_DTYPE_F32 ? 4u : dtype == YULE_DTYPE_F16 || dtype == YULE_DTYPE_BF16 ? 2u : 0u;
+}
+
+// the head size that the kernels are built for (dims past head_dim are zeros in registers and LDS)
+inline uint32_t attn_padded_dim(uint32_t hd) { return hd <= 64 ? 64u : hd <= 96 ? 96u : hd <= 128 ? 128u : 256u; }
+
+// Rows r < n_rows, each `width` elements of `elem` bytes, of a buffer of
+// buf_bytes: nullptr, or what is wrong.  align: bytes that every row starts at
+// a multiple of.  Row offsets inside 32 rows have to fit 31 bits (the copies
+// into LDS take 32-bit offsets from a 64-bit row address).
+inline const char *check_rows(uint64_t offset, uint64_t stride, uint64_t n_rows, uint64_t width, uint32_t elem,
+                              uint64_t buf_bytes, uint32_t align) {
+    if (!n_rows || !width) return nullptr;
+    const uint64_t elems = buf_bytes / elem;
+    if (stride < width && n_rows > 1) return "rows overlap (stride below the row's width)";
+    if (stride >= (uint64_t)1 << 24) return "row stride of 2^24 elements or more";
+    if (width > elems || offset > elems - width) return "rows reach past the buffer";
+    if (n_rows > 1 && (elems - width - offset) / stride < n_rows - 1) return "rows reach past the buffer";
+    if ((offset * elem) % align || (n_rows > 1 && (stride * elem) % align)) return "rows are not aligned";
+    return nullptr;
+}
+
+// heads and types of an attention call: nullptr, or what is wrong
+inline const char *check_heads(uint32_t n_heads, uint32_t n_kv, uint32_t hd) {
+    if (!n_heads || !n_kv || n_heads % n_kv) return "n_heads must be a positive multiple of n_kv_heads";
+    if (!hd || hd % 8 || hd > 256) return "head_dim must be a multiple of 8, at most 256";
+    if (n_heads > 4096) return "more than 4096 heads";
+    return nullptr;
+}
+
+// (query rows x heads per KV head) of one wave's tile
+constexpr uint32_t kAttnTileRows = 32;
+// workgroups of one launch: its threads count in 32 bits
+constexpr uint64_t kMaxWorkgroups = (uint64_t)1 << 23;
+constexpr uint32_t kMaxKeys = 1u << 30;   // of a prefix, and of a tail
+
+// ---- verify_drafts: values of a row per workgroup, and what a chunk leaves
+// (f64 sums of max(p - q, 0) and of p, and the last places where they are not 0)
+constexpr uint32_t kVerifyChunk = 4096, kMaxVocab = 1u << 30, kMaxDrafts = 1024;
+struct VerifySum {
+    double rest, whole;
+    int last_rest, last_whole;
+};
+
+// ---- prefix_attn: the prefix and each tail in chunks of keys, one workgroup
+// each; a chunk's results (unnormalised sums, maximum and weight of the softmax)
+// go to the workspace and are joined by a second launch.
+struct PrefixPlan {
+    uint32_t p_chunk, n_p;   // keys of a prefix chunk, chunks (0 without a prefix)
+    uint32_t t_chunk, n_t;   // the same of a tail
+    uint32_t p_tiles, t_tiles;   // query tiles per KV head over the whole batch, and per sequence
+    uint64_t rows;           // (query row, head) pairs
+    uint64_t p_jobs, t_jobs;
+    size_t ml_bytes, o_bytes;   // workspace: (m, l) pairs, then the sums
+
+    size_t bytes() const { return ml_bytes + o_bytes; }
+    // indexes of a chunk's (m, l) pair and of its sums
+    uint64_t ml_at(uint32_t chunk, uint64_t row) const { return chunk * rows + row; }
+};
+
+inline PrefixPlan prefix_plan(uint32_t prefix_len, uint32_t tail_cap, uint32_t n_seqs, uint32_t n_tokens,
+                              uint32_t n_heads, uint32_t n_kv, uint32_t hd, uint32_t cus) {
+    PrefixPlan p{};
+    const uint64_t group = n_heads / n_kv, slots = (uint64_t)n_seqs * n_tokens * group;
+    p.p_tiles = (uint32_t)((slots + kAttnTileRows - 1) / kAttnTileRows);
+    p.t_tiles = (uint32_t)((n_tokens * group + kAttnTileRows - 1) / kAttnTileRows);
+    // enough chunks for two workgroups a CU, none below 256 keys (two tiles of every wave)
+    auto split = [&](uint32_t keys, uint64_t per_chunk, uint32_t *chunk, uint32_t *n) {
+        if (!keys) return;
+        uint64_t want = (2ull * cus + per_chunk - 1) / per_chunk;
+        const uint64_t most = (keys + 255) / 256;
+        if (want > most) want = most;
+        *chunk = (uint32_t)((((uint64_t)keys + want - 1) / want + 127) / 128 * 128);
+        *n = (uint32_t)(((uint64_t)keys + *chunk - 1) / *chunk);
+    };
+    split(prefix_len, (uint64_t)p.p_tiles * n_kv, &p.p_chunk, &p.n_p);
+    split(tail_cap, (uint64_t)p.t_tiles * n_kv * n_seqs, &p.t_chunk, &p.n_t);
+    p.rows = (uint64_t)n_seqs * n_tokens * n_heads;
+    p.p_jobs = (uint64_t)p.n_p * p.p_tiles * n_kv;
+    p.t_jobs = (uint64_t)p.n_t * p.t_tiles * n_kv * n_seqs;
+    const uint64_t parts = (uint64_t)(p.n_p + p.n_t) * p.rows;
+    p.ml_bytes = (size_t)((parts * 8 + 255) / 256 * 256);
+    p.o_bytes = (size_t)(parts * hd * 4);
+    return p;
+}
+
+}  // namespace yule

@@ -8,6 +8,7 @@
 #include <mutex>
 #include <string>
 #include <unordered_map>
+#include <vector>
 
 #include "../../include/yule_hip.h"
 
@@ -42,6 +43,10 @@ struct yule_hip_backend {
     std::mutex scratch_mu;
     void *scratch = nullptr;
     size_t scratch_size = 0;
+    // a graph captured with the present workspace may be replayed after it has
+    // grown: such a workspace is kept until the backend ends
+    bool scratch_in_graph = false;
+    std::vector<void *> scratch_kept;
     // argmax's workgroup slots and ticket: allocated and zeroed at creation,
     // left zeroed by every launch on the backend's one stream
     void *argmax_ws = nullptr;
@@ -56,6 +61,33 @@ int hip_error(hipError_t e, const char *what);
 // Look up a handle and check that [offset, offset+need) lies inside it.
 int get_buffer(yule_hip_backend *be, uint64_t h, size_t need, void **ptr, const char *what,
                size_t offset = 0);
+
+// Rows r < n_rows of an argument of a batched operator, `width` elements of
+// `elem` bytes each: address of the first (align: what every row starts at a
+// multiple of), or the refusal.
+int rows_ptr(yule_hip_backend *be, const yule_rows *r, uint64_t n_rows, uint64_t width, uint32_t elem, uint32_t align,
+             const char *what, void **ptr);
+
+// A C entry's body: with the backend's device current (the caller's is put
+// back), and with C++ exceptions turned into an error.
+template <typename F>
+int guarded(const char *what, yule_hip_backend *be, F body) {
+    try {
+        if (!be) return set_error(YULE_ERR_INVALID, "null backend");
+        int was = be->device, rc;
+        if ((rc = hip_error(hipGetDevice(&was), what))) return rc;
+        if (was != be->device && (rc = hip_error(hipSetDevice(be->device), what))) return rc;
+        struct Back {
+            int was, now;
+            ~Back() {
+                if (was != now) (void)hipSetDevice(was);
+            }
+        } back{was, be->device};
+        return body();
+    } catch (...) {   // (an allocation of the host's)
+        return YULE_ERR_OOM;
+    }
+}
 
 // The backend's workspace for one call.  The lease holds the workspace lock
 // until it is destroyed, so a call enqueues every launch that uses the

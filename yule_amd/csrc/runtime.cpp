@@ -12,6 +12,7 @@
 #include <string>
 #include <vector>
 
+#include "batch_plan.h"
 #include "internal.h"
 
 namespace {
@@ -50,23 +51,26 @@ int workspace_alloc(size_t bytes, void **p, const char *what) {
 
 int get_scratch(yule_hip_backend *be, size_t need, ScratchLease *lease) {
     std::unique_lock<std::mutex> lk(be->scratch_mu);
+    int rc;
+    hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
+    if ((rc = hip_error(hipStreamIsCapturing(be->stream, &cap), "scratch: capture status"))) return rc;
     if (be->scratch_size < need) {
-        int rc;
         // neither the wait nor the allocation can be captured, and trying would spoil the capture
-        hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
-        if ((rc = hip_error(hipStreamIsCapturing(be->stream, &cap), "scratch: capture status"))) return rc;
         if (cap != hipStreamCaptureStatusNone)
             return set_error(YULE_ERR_HIP, "scratch: cannot grow under stream capture");
         if (be->scratch) {
             if ((rc = hip_error(hipStreamSynchronize(be->stream), "scratch: synchronize"))) return rc;
-            (void)hipFree(be->scratch);
+            if (be->scratch_in_graph) be->scratch_kept.push_back(be->scratch);
+            else (void)hipFree(be->scratch);
             be->scratch = nullptr;
             be->scratch_size = 0;
+            be->scratch_in_graph = false;
         }
         const size_t sz = (need + ((size_t)1 << 20) - 1) & ~(((size_t)1 << 20) - 1);
         if ((rc = workspace_alloc(sz, &be->scratch, "scratch: allocate"))) return rc;
         be->scratch_size = sz;
     }
+    if (cap != hipStreamCaptureStatusNone) be->scratch_in_graph = true;
     lease->ptr = be->scratch;
     lease->lock = std::move(lk);
     return YULE_OK;
@@ -83,6 +87,19 @@ int get_buffer(yule_hip_backend *be, uint64_t h, size_t need, void **ptr, const 
                                                " exceeds buffer " + std::to_string(h) + " of " +
                                                std::to_string(it->second.size) + " bytes");
     *ptr = static_cast<uint8_t *>(it->second.ptr) + offset;
+    return YULE_OK;
+}
+
+int rows_ptr(yule_hip_backend *be, const yule_rows *r, uint64_t n_rows, uint64_t width, uint32_t elem, uint32_t align,
+             const char *what, void **ptr) {
+    if (!r) return set_error(YULE_ERR_INVALID, std::string(what) + ": null rows");
+    std::lock_guard<std::mutex> lk(be->mu);
+    auto it = be->buffers.find(r->buffer);
+    if (it == be->buffers.end())
+        return set_error(YULE_ERR_INVALID, std::string(what) + ": buffer " + std::to_string(r->buffer) + " not found");
+    if (const char *bad = check_rows(r->offset, r->stride, n_rows, width, elem, it->second.size, align))
+        return set_error(YULE_ERR_INVALID, std::string(what) + ": " + bad);
+    *ptr = static_cast<uint8_t *>(it->second.ptr) + (n_rows && width ? r->offset * elem : 0);
     return YULE_OK;
 }
 
@@ -169,6 +186,7 @@ int yule_hip_destroy(yule_hip_backend *be) {
     for (auto &kv : be->buffers) hipFree(kv.second.ptr);
     be->buffers.clear();
     if (be->scratch) hipFree(be->scratch);
+    for (void *p : be->scratch_kept) hipFree(p);
     if (be->argmax_ws) hipFree(be->argmax_ws);
     for (hipEvent_t e : be->timer)
         if (e) hipEventDestroy(e);

@@ -5,7 +5,7 @@ from enum import IntEnum
 
 
 class DType(IntEnum):
-    """GGUF type ids, dtype.rs:21-35 (the values cross the C ABI)."""
+    """GGUF type ids, dtype.rs:21-35 (the values cross the C ABI); BF16 is the file format's own id."""
     F32 = 0
     F16 = 1
     Q4_0 = 2
@@ -14,6 +14,7 @@ class DType(IntEnum):
     Q5_K = 13
     Q6_K = 14
     Q8_K = 15
+    BF16 = 30
 
 
 # (weights per block, bytes per block): dtype.rs:62-118
