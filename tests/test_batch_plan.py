@@ -53,6 +53,7 @@ int main() {
         CHECK(p.rows == (uint64_t)seqs * tokens * kv * group);
         CHECK((uint64_t)p.p_chunk * p.n_p >= prefix && (!p.n_p || (uint64_t)p.p_chunk * (p.n_p - 1) < prefix));
         CHECK((uint64_t)p.t_chunk * p.n_t >= cap && (!p.n_t || (uint64_t)p.t_chunk * (p.n_t - 1) < cap));
+        CHECK(p.n_p + p.n_t <= kMaxParts);
         CHECK((prefix == 0) == (p.n_p == 0) && (cap == 0) == (p.n_t == 0));
         CHECK((uint64_t)p.p_tiles * kAttnTileRows >= (uint64_t)seqs * tokens * group);
         CHECK((uint64_t)p.t_tiles * kAttnTileRows >= (uint64_t)tokens * group);

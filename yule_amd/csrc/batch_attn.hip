@@ -532,31 +532,64 @@ __global__ __launch_bounds__((64 * BlockAttn<T, D>::NW))
            });
 }
 
-// out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c over a row's chunks, a wave
-// per (row, head).  A row that saw no key has l = 0 everywhere and gives zeros.
-template <typename T>
-__global__ __launch_bounds__(256) void prefix_join_kernel(const float2 *__restrict__ ml, const float *__restrict__ o,
-                                                          uint8_t *__restrict__ out, uint32_t os, uint32_t rows,
-                                                          uint32_t n_heads, uint32_t hd, uint32_t parts) {
-    const uint32_t at = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63u;
-    if (at >= rows) return;
+// out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c over a row's chunks, a
+// workgroup per (row, head): its threads take the chunks' factors together, then
+// groups of G lanes (four dims each) take the chunks in turn, so that their
+// loads do not wait for each other.  A row that saw no key has l = 0 everywhere
+// and gives zeros.
+template <typename T, uint32_t NT, uint32_t G>
+__global__ __launch_bounds__(NT) void prefix_join_kernel(const float2 *__restrict__ ml, const float *__restrict__ o,
+                                                         uint8_t *__restrict__ out, uint32_t os, uint32_t rows,
+                                                         uint32_t n_heads, uint32_t hd, uint32_t parts) {
+    constexpr uint32_t NG = NT / G, NW = NT / 64;
+    __shared__ float f[kMaxParts];   // a chunk's factor; -1: it saw no key, and its sums were not written
+    __shared__ float red[2][NW];
+    __shared__ f4v sums[NG][G];
+    const uint32_t at = blockIdx.x, tid = threadIdx.x, lane = tid & 63u, g = tid / G, d = 4 * (tid % G);
     float M = -INFINITY;
-    for (uint32_t p = lane; p < parts; p += 64) M = fmaxf(M, ml[(size_t)p * rows + at].x);
+    for (uint32_t p = tid; p < parts; p += NT) M = fmaxf(M, ml[(size_t)p * rows + at].x);
 #pragma unroll
-    for (uint32_t d = 32; d; d /= 2) M = fmaxf(M, __shfl_xor(M, d, 64));
-    float L = 0.f;
-    f4v acc = {0.f, 0.f, 0.f, 0.f};
-    for (uint32_t p = 0; p < parts; p++) {
-        const float2 x = ml[(size_t)p * rows + at];
-        if (x.x == -INFINITY && x.y == 0.f) continue;   // no key of this chunk: its sums were not written
-        const float f = __builtin_amdgcn_exp2f(x.x - M);
-        L += f * x.y;
-        if (4 * lane < hd) acc += f * *reinterpret_cast<const f4v *>(o + ((size_t)p * rows + at) * hd + 4 * lane);
+    for (uint32_t x = 32; x; x /= 2) M = fmaxf(M, __shfl_xor(M, x, 64));
+    if (NW > 1) {
+        if (lane == 0) red[0][tid >> 6] = M;
+        __syncthreads();
+#pragma unroll
+        for (uint32_t w = 0; w < NW; w++) M = fmaxf(M, red[0][w]);
     }
-    const float inv = L == 0.f ? 0.f : 1.0f / L;
-    const uint32_t row = at / n_heads;
-    if (4 * lane < hd)
-        store4<T>(out + (size_t)row * os + (size_t)(at - row * n_heads) * hd * sizeof(T), 4 * lane, acc * inv);
+    float L = 0.f;
+    for (uint32_t p = tid; p < parts; p += NT) {
+        const float2 x = ml[(size_t)p * rows + at];
+        const bool none = x.x == -INFINITY && x.y == 0.f;
+        const float e = none ? -1.f : __builtin_amdgcn_exp2f(x.x - M);
+        f[p] = e;
+        if (!none) L += e * x.y;
+    }
+#pragma unroll
+    for (uint32_t x = 32; x; x /= 2) L += __shfl_xor(L, x, 64);
+    if (lane == 0) red[1][tid >> 6] = L;
+    __syncthreads();
+    f4v acc = {0.f, 0.f, 0.f, 0.f};
+    if (d < hd) {
+        const float *mine = o + (size_t)at * hd + d;
+        const size_t step = (size_t)rows * hd;
+#pragma unroll 4
+        for (uint32_t p = g; p < parts; p += NG) {
+            const float e = f[p];
+            if (e != -1.f) acc += e * *reinterpret_cast<const f4v *>(mine + p * step);
+        }
+    }
+    sums[g][tid % G] = acc;
+    __syncthreads();
+    if (tid < G && d < hd) {
+        L = 0.f;
+#pragma unroll
+        for (uint32_t w = 0; w < NW; w++) L += red[1][w];
+        acc = sums[0][tid];
+#pragma unroll
+        for (uint32_t i = 1; i < NG; i++) acc += sums[i][tid];
+        const uint32_t row = at / n_heads;
+        store4<T>(out + (size_t)row * os + (size_t)(at - row * n_heads) * hd * sizeof(T), d, acc * (L == 0.f ? 0.f : 1.0f / L));
+    }
 }
 
 // f(element type, padded head size)
@@ -598,14 +631,16 @@ static int launch_prefix(hipStream_t s, const PrefixArgs &a, uint32_t dtype, uin
 }
 
 static int launch_join(hipStream_t s, const PrefixArgs &a, uint8_t *out, uint32_t os, uint32_t dtype) {
-    const uint32_t n_heads = a.s.group * a.s.n_kv, rows = a.n_seqs * a.n_tokens * n_heads;
-    auto go = [&](auto t) {
-        hipLaunchKernelGGL((prefix_join_kernel<decltype(t)>), dim3((rows + 3) / 4), dim3(256), 0, s, a.ml, a.o, out, os,
-                           rows, n_heads, a.s.hd, a.n_p + a.n_t);
-    };
-    if (dtype == YULE_DTYPE_F32) go(float{});
-    else if (dtype == YULE_DTYPE_F16) go((_Float16)0);
-    else go((__bf16)0);
+    const uint32_t n_heads = a.s.group * a.s.n_kv, rows = a.n_seqs * a.n_tokens * n_heads, hd = a.s.hd, parts = a.n_p + a.n_t;
+    by_shape(dtype, hd, [&](auto t, auto d) {
+        using T = decltype(t);
+        constexpr uint32_t D = decltype(d)::value, G = D <= 64 ? 16 : D <= 128 ? 32 : 64;
+        // one wave where it takes every chunk in a step or two
+        if (parts <= 2 * 64 / G)
+            hipLaunchKernelGGL((prefix_join_kernel<T, 64, G>), dim3(rows), dim3(64), 0, s, a.ml, a.o, out, os, rows, n_heads, hd, parts);
+        else
+            hipLaunchKernelGGL((prefix_join_kernel<T, 256, G>), dim3(rows), dim3(256), 0, s, a.ml, a.o, out, os, rows, n_heads, hd, parts);
+    });
     return check_launch("prefix_attn (join)");
 }
 
@@ -697,7 +732,7 @@ int yule_hip_prefix_attn(yule_hip_backend *be, const yule_rows *q, const yule_ro
         if (!n_seqs) return YULE_OK;
         const PrefixPlan p = prefix_plan(prefix_len, tail_cap, n_seqs, n_tokens, n_heads, n_kv_heads, head_dim,
                                          (uint32_t)be->props.multiProcessorCount);
-        if (p.rows >= (uint64_t)1 << 25 || p.p_jobs + p.t_jobs > kMaxWorkgroups)
+        if (p.rows > kMaxWorkgroups || p.p_jobs + p.t_jobs > kMaxWorkgroups)
             return set_error(YULE_ERR_INVALID, "prefix_attn: too many rows for one call");
         ScratchLease ws;   // held until both launches are enqueued
         if ((rc = get_scratch(be, p.bytes(), &ws))) return rc;

@@ -53,10 +53,14 @@ constexpr uint32_t kMaxKeys = 1u << 30;   // of a prefix, and of a tail
 // ---- verify_drafts: values of a row per workgroup, and what a chunk leaves
 // (f64 sums of max(p - q, 0) and of p, and the last places where they are not 0)
 constexpr uint32_t kVerifyChunk = 4096, kMaxVocab = 1u << 30, kMaxDrafts = 1024;
+constexpr uint32_t kVerifyTickets = 4096;   // sequences of one launch
 struct VerifySum {
     double rest, whole;
     int last_rest, last_whole;
 };
+
+// chunks of a prefix and a tail together
+constexpr uint32_t kMaxParts = 1024;
 
 // ---- prefix_attn: the prefix and each tail in chunks of keys, one workgroup
 // each; a chunk's results (unnormalised sums, maximum and weight of the softmax)
@@ -86,6 +90,7 @@ inline PrefixPlan prefix_plan(uint32_t prefix_len, uint32_t tail_cap, uint32_t n
         uint64_t want = (2ull * cus + per_chunk - 1) / per_chunk;
         const uint64_t most = (keys + 255) / 256;
         if (want > most) want = most;
+        if (want > kMaxParts / 2) want = kMaxParts / 2;
         *chunk = (uint32_t)((((uint64_t)keys + want - 1) / want + 127) / 128 * 128);
         *n = (uint32_t)(((uint64_t)keys + *chunk - 1) / *chunk);
     };

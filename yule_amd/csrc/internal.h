@@ -50,6 +50,8 @@ struct yule_hip_backend {
     // argmax's workgroup slots and ticket: allocated and zeroed at creation,
     // left zeroed by every launch on the backend's one stream
     void *argmax_ws = nullptr;
+    // verify_drafts' tickets, a u32 a sequence: kept the same way
+    void *verify_ws = nullptr;
 };
 
 namespace yule {

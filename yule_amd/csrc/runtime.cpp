@@ -171,7 +171,9 @@ int yule_hip_create(int device, yule_hip_backend **out) {
         return rc;
     }
     if ((rc = hip_error(hipMalloc(&be->argmax_ws, argmax_ws_bytes()), "create: argmax workspace")) ||
-        (rc = hip_error(hipMemsetAsync(be->argmax_ws, 0, argmax_ws_bytes(), be->stream), "create: argmax workspace"))) {
+        (rc = hip_error(hipMemsetAsync(be->argmax_ws, 0, argmax_ws_bytes(), be->stream), "create: argmax workspace")) ||
+        (rc = hip_error(hipMalloc(&be->verify_ws, kVerifyTickets * 4), "create: verify tickets")) ||
+        (rc = hip_error(hipMemsetAsync(be->verify_ws, 0, kVerifyTickets * 4, be->stream), "create: verify tickets"))) {
         yule_hip_destroy(be);
         return rc;
     }
@@ -188,6 +190,7 @@ int yule_hip_destroy(yule_hip_backend *be) {
     if (be->scratch) hipFree(be->scratch);
     for (void *p : be->scratch_kept) hipFree(p);
     if (be->argmax_ws) hipFree(be->argmax_ws);
+    if (be->verify_ws) hipFree(be->verify_ws);
     for (hipEvent_t e : be->timer)
         if (e) hipEventDestroy(e);
     if (be->cap_exec) hipGraphExecDestroy(be->cap_exec);

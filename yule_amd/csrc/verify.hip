@@ -10,9 +10,9 @@
 //
 // One row of p and one of q is all that has to be read (the drafts' own
 // probabilities besides): bandwidth for a batch, latency for a single request.
-// The rows are cut into chunks of 4096 values, one workgroup each, which leave
-// their sums; a second launch finds the chunk that the pick falls into and walks
-// that one again.
+// One launch: the rows are cut into chunks of 4096 values, a workgroup each,
+// which leave their sums; the workgroup that takes a sequence's last ticket finds
+// the chunk that the pick falls into and walks that one again.
 #include <cmath>
 
 #include "batch_plan.h"
@@ -27,8 +27,9 @@ struct VerifyArgs {
     const float *u;              // [n_seqs][n_draft + 1]
     const uint32_t *lens;        // drafts of each sequence, or null
     uint32_t *accepted, *tokens; // [n_seqs], [n_seqs][n_draft + 1]
-    uint32_t n_draft, vocab, chunks;
-    VerifySum *sums;             // [n_seqs][chunks]
+    uint32_t n_draft, vocab, chunks, seq0;
+    VerifySum *sums;             // [sequences of the launch][chunks]
+    uint32_t *tickets;           // [sequences of the launch], zero before and after
 };
 
 // a weight: what is not a positive number counts as nothing
@@ -79,108 +80,220 @@ __device__ __forceinline__ int wave_max(int x) {
     return x;
 }
 
-__global__ __launch_bounds__(256) void verify_sums_kernel(VerifyArgs a) {
-    __shared__ double sr[4], sp[4];
-    __shared__ int lr[4], lp[4];
-    const uint32_t s = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks, tid = threadIdx.x, lane = tid & 63u;
-    uint32_t count;
-    const uint32_t n = kept(a, s, lane, &count);
-    const float *p, *q;
-    rows_of(a, s, n, count, &p, &q);
-    const uint32_t x0 = chunk * kVerifyChunk, x1 = a.vocab - x0 < kVerifyChunk ? a.vocab : x0 + kVerifyChunk;
-    double rest = 0.0, whole = 0.0;   // of max(p - q, 0), of p
-    int last_rest = -1, last_whole = -1;
-    for (uint32_t x = x0 + tid; x < x1; x += 256) {
-        const double pv = p[x], w = weight(pv), r = q ? weight(pv - (double)q[x]) : w;
-        rest += r;
-        whole += w;
-        if (r > 0.0) last_rest = (int)x;
-        if (w > 0.0) last_whole = (int)x;
-    }
-    rest = wave_sum(rest);
-    whole = wave_sum(whole);
-    last_rest = wave_max(last_rest);
-    last_whole = wave_max(last_whole);
-    if (lane == 0) {
-        sr[tid >> 6] = rest, sp[tid >> 6] = whole;
-        lr[tid >> 6] = last_rest, lp[tid >> 6] = last_whole;
-    }
-    __syncthreads();
-    if (tid == 0) {
-        VerifySum v = {sr[0], sp[0], lr[0], lp[0]};
-        for (int i = 1; i < 4; i++) {
-            v.rest += sr[i];
-            v.whole += sp[i];
-            v.last_rest = lr[i] > v.last_rest ? lr[i] : v.last_rest;
-            v.last_whole = lp[i] > v.last_whole ? lp[i] : v.last_whole;
+// Values x0 + 1024 j + 4 tid + e (j, e < 4) of a row in this thread's registers,
+// 0 past n: 16-byte loads where the row allows them.
+__device__ __forceinline__ void load_chunk(const float *row, uint32_t x0, uint32_t n, uint32_t tid, float v[4][4]) {
+    const bool whole = x0 + kVerifyChunk <= n && (reinterpret_cast<uintptr_t>(row) & 15u) == 0;
+    if (whole) {
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) {
+            const float4 f = *reinterpret_cast<const float4 *>(row + x0 + 1024 * j + 4 * tid);
+            v[j][0] = f.x, v[j][1] = f.y, v[j][2] = f.z, v[j][3] = f.w;
         }
-        a.sums[blockIdx.x] = v;
+    } else {
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++)
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++) {
+                const uint32_t x = x0 + 1024 * j + 4 * tid + e;
+                const float f = row[x < n ? x : n - 1u];
+                v[j][e] = x < n ? f : 0.f;
+            }
     }
 }
 
-// a workgroup per sequence
-__global__ __launch_bounds__(256) void verify_pick_kernel(VerifyArgs a) {
-    __shared__ double part[256];
-    __shared__ uint32_t found;
-    const uint32_t s = blockIdx.x, tid = threadIdx.x, lane = tid & 63u;
+// inclusive sums over the wave's lanes
+__device__ __forceinline__ double wave_scan(double x, uint32_t lane) {
+#pragma unroll
+    for (uint32_t d = 1; d < 64; d *= 2) {
+        const double y = __shfl_up(x, d, 64);
+        if (lane >= d) x += y;
+    }
+    return x;
+}
+
+// A workgroup per chunk; the one that takes its sequence's last ticket picks and
+// answers.  Sums are taken in one order, whoever is last.
+__global__ __launch_bounds__(256) void verify_kernel(VerifyArgs a) {
+    __shared__ double part[2][16];   // sums of max(p - q, 0), of p, of 256 values each: 1024 j + 256 wave ..
+    __shared__ int lasts[2][4];      // last places where they are not 0, by wave
+    __shared__ double target, before;
+    __shared__ uint32_t is_last, at, of_rest, token;
+    const uint32_t s = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks, seq = a.seq0 + s;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
     uint32_t count;
-    const uint32_t n = kept(a, s, lane, &count);
+    const uint32_t n = kept(a, seq, lane, &count);
     const float *p, *q;
-    rows_of(a, s, n, count, &p, &q);
-    const VerifySum *sums = a.sums + (size_t)s * a.chunks;
-    // every thread walks the chunks in order: the same additions everywhere
-    double rest = 0.0, whole = 0.0;
-    for (uint32_t c = 0; c < a.chunks; c++) {
-        rest += sums[c].rest;
-        whole += sums[c].whole;
-    }
-    const bool of_rest = rest > 0.0;   // (rounding may leave p = q at a draft that is not kept: then p itself)
-    const double target = (double)a.u[(size_t)s * (a.n_draft + 1) + a.n_draft] * (of_rest ? rest : whole);
-    double sum = 0.0;
-    uint32_t at = a.chunks;
-    int last = -1;
-    for (uint32_t c = 0; c < a.chunks; c++) {
-        const double w = of_rest ? sums[c].rest : sums[c].whole;
-        const int l = of_rest ? sums[c].last_rest : sums[c].last_whole;
-        if (l >= 0) last = l;
-        if (sum + w > target) {
-            at = c;
-            break;
+    rows_of(a, seq, n, count, &p, &q);
+
+    double r[4][4], w[4][4];   // this thread's weights of a chunk
+    auto weigh = [&](uint32_t x0) {
+        float pv[4][4], qv[4][4];
+        load_chunk(p, x0, a.vocab, tid, pv);
+        if (q) load_chunk(q, x0, a.vocab, tid, qv);
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++) {
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++) {
+                w[j][e] = weight(pv[j][e]);
+                r[j][e] = q ? weight((double)pv[j][e] - (double)qv[j][e]) : w[j][e];
+            }
+            const double sr = wave_sum((r[j][0] + r[j][1]) + (r[j][2] + r[j][3]));
+            const double sw = q ? wave_sum((w[j][0] + w[j][1]) + (w[j][2] + w[j][3])) : sr;
+            if (lane == 0) part[0][4 * j + wave] = sr, part[1][4 * j + wave] = sw;
         }
-        sum += w;
-    }
-    // (not passed at all: u or a rounding at the very end; the last token that has a weight.  None has: no token)
-    uint32_t token = last < 0 ? YULE_NO_TOKEN : (uint32_t)last;
-    if (at < a.chunks) {
-        const uint32_t x0 = at * kVerifyChunk, x1 = a.vocab - x0 < kVerifyChunk ? a.vocab : x0 + kVerifyChunk;
-        constexpr uint32_t EACH = kVerifyChunk / 256;
-        auto w_of = [&](uint32_t x) {
-            if (x >= x1) return 0.0;
-            const double pv = p[x];
-            return of_rest && q ? weight(pv - (double)q[x]) : weight(pv);
-        };
-        double mine = 0.0;
-        for (uint32_t i = 0; i < EACH; i++) mine += w_of(x0 + tid * EACH + i);
-        part[tid] = mine;
-        if (tid == 0) found = token;   // (last weighted token of the chunk, should its sum round below the target)
-        __syncthreads();
-        for (uint32_t i = 0; i < tid; i++) sum += part[i];
-        __syncthreads();
-        for (uint32_t i = 0; i < EACH && mine > 0.0; i++) {
-            sum += w_of(x0 + tid * EACH + i);
-            if (sum > target) {
-                atomicMin(&found, x0 + tid * EACH + i);
-                break;
+    };
+    weigh(chunk * kVerifyChunk);
+    int last_r = -1, last_w = -1;
+#pragma unroll
+    for (uint32_t j = 0; j < 4; j++)
+#pragma unroll
+        for (uint32_t e = 0; e < 4; e++) {
+            const int x = (int)(chunk * kVerifyChunk + 1024 * j + 4 * tid + e);
+            if (r[j][e] > 0.0) last_r = x;
+            if (w[j][e] > 0.0) last_w = x;
+        }
+    last_r = wave_max(last_r);
+    last_w = wave_max(last_w);
+    if (lane == 0) lasts[0][wave] = last_r, lasts[1][wave] = last_w;
+    __syncthreads();
+
+    // the first wave: this chunk's sums out, the ticket; with the last one the
+    // chunk that the pick falls into, 64 chunks at a time
+    if (wave == 0) {
+        VerifySum v = {0.0, 0.0, -1, -1};
+#pragma unroll
+        for (uint32_t i = 0; i < 16; i++) {
+            v.rest += part[0][i];
+            v.whole += part[1][i];
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < 4; i++) {
+            v.last_rest = lasts[0][i] > v.last_rest ? lasts[0][i] : v.last_rest;
+            v.last_whole = lasts[1][i] > v.last_whole ? lasts[1][i] : v.last_whole;
+        }
+        uint32_t mine = 1;
+        if (a.chunks > 1) {
+            if (lane == 0) {
+                // complete at device scope before the ticket is taken (no cache-wide fence)
+                uint64_t *o = reinterpret_cast<uint64_t *>(a.sums + blockIdx.x);
+                const uint64_t words[3] = {__builtin_bit_cast(uint64_t, v.rest), __builtin_bit_cast(uint64_t, v.whole),
+                                           (uint64_t)(uint32_t)v.last_whole << 32 | (uint32_t)v.last_rest};
+#pragma unroll
+                for (int i = 0; i < 3; i++) __hip_atomic_store(o + i, words[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                __atomic_signal_fence(__ATOMIC_SEQ_CST);
+                __builtin_amdgcn_s_waitcnt(0);
+                __atomic_signal_fence(__ATOMIC_SEQ_CST);
+                mine = __hip_atomic_fetch_add(a.tickets + s, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.chunks - 1u;
+                if (mine) __hip_atomic_store(a.tickets + s, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            mine = __builtin_amdgcn_readfirstlane(mine);
+        }
+        if (lane == 0) is_last = mine;
+        if (mine) {
+            __atomic_signal_fence(__ATOMIC_SEQ_CST);
+            double c_rest, c_whole;   // sums of lane's chunk (this one's own without others), their last places
+            int c_lr, c_lw;
+            auto load_sums = [&](uint32_t c) {
+                c_rest = c_whole = 0.0;
+                c_lr = c_lw = -1;
+                if (a.chunks == 1) {
+                    if (c == 0) c_rest = v.rest, c_whole = v.whole, c_lr = v.last_rest, c_lw = v.last_whole;
+                } else if (c < a.chunks) {
+                    const uint64_t *o = reinterpret_cast<const uint64_t *>(a.sums + (size_t)s * a.chunks + c);
+                    c_rest = __builtin_bit_cast(double, __hip_atomic_load(o, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+                    c_whole = __builtin_bit_cast(double, __hip_atomic_load(o + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+                    const uint64_t l = __hip_atomic_load(o + 2, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    c_lr = (int)(uint32_t)l;
+                    c_lw = (int)(uint32_t)(l >> 32);
+                }
+            };
+            double all_rest = 0.0, all_whole = 0.0;
+            int all_lr = -1, all_lw = -1;
+            for (uint32_t c0 = 0; c0 < a.chunks; c0 += 64) {
+                load_sums(c0 + lane);
+                all_rest += wave_sum(c_rest);
+                all_whole += wave_sum(c_whole);
+                const int lr = wave_max(c_lr), lw = wave_max(c_lw);
+                all_lr = lr > all_lr ? lr : all_lr;
+                all_lw = lw > all_lw ? lw : all_lw;
+            }
+            const bool rest = all_rest > 0.0;   // (rounding may leave p = q at a draft that is not kept: then p itself)
+            const double t = (double)a.u[(size_t)seq * (a.n_draft + 1) + a.n_draft] * (rest ? all_rest : all_whole);
+            double sum = 0.0;
+            uint32_t hit = a.chunks;
+            for (uint32_t c0 = 0; c0 < a.chunks; c0 += 64) {
+                if (a.chunks > 64) load_sums(c0 + lane);
+                const double upto = wave_scan(rest ? c_rest : c_whole, lane);
+                const uint64_t past = __ballot(c0 + lane < a.chunks && sum + upto > t);
+                if (past) {
+                    const int l = __builtin_ctzll(past);
+                    hit = c0 + (uint32_t)l;
+                    const double up = __shfl(upto, l ? l - 1 : 0, 64);
+                    if (l) sum += up;
+                    break;
+                }
+                sum += __shfl(upto, 63, 64);
+            }
+            if (lane == 0) {
+                // not passed at all (u, or a rounding, at the very end): the last token that has a weight, if one has
+                const int l = rest ? all_lr : all_lw;
+                token = l < 0 ? YULE_NO_TOKEN : (uint32_t)l;
+                target = t, before = sum, at = hit, of_rest = rest;
             }
         }
-        __syncthreads();
-        token = found;
     }
+    __syncthreads();
+    if (!is_last) return;
+    if (at < a.chunks) {
+        if (a.chunks > 1) weigh(at * kVerifyChunk);   // (one chunk: still there)
+        __syncthreads();
+        // the 256 values, then the four, then the value
+        const double *sums = part[of_rest ? 0 : 1];
+        // (sums taken in other orders may round to either side of the target: then the last with a weight)
+        double run_sum = before, sum = before;
+        uint32_t i = 0;
+        for (uint32_t k = 0; k < 16; k++) {
+            if (sums[k] > 0.0) {
+                i = k;
+                sum = run_sum;
+                if (run_sum + sums[k] > target) break;
+            }
+            run_sum += sums[k];
+        }
+        if (wave == (i & 3u)) {
+            double mine[4];
+#pragma unroll
+            for (uint32_t j = 0; j < 4; j++)
+                if (j == i >> 2) {
+#pragma unroll
+                    for (uint32_t e = 0; e < 4; e++) mine[e] = of_rest ? r[j][e] : w[j][e];
+                }
+            const double four = (mine[0] + mine[1]) + (mine[2] + mine[3]);
+            const double upto = sum + wave_scan(four, lane);
+            const uint64_t past = __ballot(upto > target && four > 0.0), some = __ballot(four > 0.0);
+            const uint32_t l = past ? (uint32_t)__builtin_ctzll(past) : some ? 63u - (uint32_t)__builtin_clzll(some) : 0u;
+            double run = __shfl_up(upto, 1, 64);
+            if (lane == 0) run = sum;
+            if (lane == l && some) {
+                uint32_t e = 0, pick = 0;
+                bool found = false;
+#pragma unroll
+                for (; e < 4; e++) {
+                    run += mine[e];
+                    if (mine[e] > 0.0 && !found) pick = e;
+                    found = found || run > target;
+                }
+                token = at * kVerifyChunk + 1024 * (i >> 2) + 4 * tid + pick;
+            }
+        }
+    }
+    __syncthreads();
     for (uint32_t i = tid; i <= a.n_draft; i += 256)
-        a.tokens[(size_t)s * (a.n_draft + 1) + i] = i < n    ? a.drafts[(size_t)s * a.n_draft + i]
-                                                    : i == n ? token
-                                                             : YULE_NO_TOKEN;
-    if (tid == 0) a.accepted[s] = n;
+        a.tokens[(size_t)seq * (a.n_draft + 1) + i] = i < n    ? a.drafts[(size_t)seq * a.n_draft + i]
+                                                      : i == n ? token
+                                                               : YULE_NO_TOKEN;
+    if (tid == 0) a.accepted[seq] = n;
 }
 
 }  // namespace yule
@@ -212,9 +325,9 @@ extern "C" int yule_hip_verify_drafts(yule_hip_backend *be, const yule_rows *tar
         if (accepted == tokens) return set_error(YULE_ERR_INVALID, "verify_drafts: outputs alias");
         if (!n_seqs) return YULE_OK;
         const uint64_t chunks = (vocab + kVerifyChunk - 1) / kVerifyChunk;
-        if (n_seqs * chunks > kMaxWorkgroups) return set_error(YULE_ERR_INVALID, "verify_drafts: too many rows for one call");
-        ScratchLease ws;   // held until both launches are enqueued
-        if ((rc = get_scratch(be, n_seqs * chunks * sizeof(VerifySum), &ws))) return rc;
+        if ((uint64_t)n_seqs * chunks > kMaxWorkgroups) return set_error(YULE_ERR_INVALID, "verify_drafts: too many rows for one call");
+        ScratchLease ws;   // held until the launches are enqueued
+        if ((rc = get_scratch(be, (n_seqs < kVerifyTickets ? n_seqs : kVerifyTickets) * chunks * sizeof(VerifySum), &ws))) return rc;
         a.p = static_cast<const float *>(pp), a.q = static_cast<const float *>(pq);
         a.ps = target->stride, a.qs = n_draft ? draft->stride : 0;
         a.drafts = static_cast<const uint32_t *>(pd), a.u = static_cast<const float *>(pu);
@@ -222,9 +335,13 @@ extern "C" int yule_hip_verify_drafts(yule_hip_backend *be, const yule_rows *tar
         a.accepted = static_cast<uint32_t *>(pa), a.tokens = static_cast<uint32_t *>(pt);
         a.n_draft = n_draft, a.vocab = vocab, a.chunks = (uint32_t)chunks;
         a.sums = static_cast<VerifySum *>(ws.ptr);
-        hipLaunchKernelGGL(verify_sums_kernel, dim3((uint32_t)(n_seqs * chunks)), dim3(256), 0, be->stream, a);
-        if ((rc = check_launch("verify_drafts (sums)"))) return rc;
-        hipLaunchKernelGGL(verify_pick_kernel, dim3(n_seqs), dim3(256), 0, be->stream, a);
-        return check_launch("verify_drafts (pick)");
+        a.tickets = static_cast<uint32_t *>(be->verify_ws);
+        for (uint32_t s0 = 0; s0 < n_seqs; s0 += kVerifyTickets) {   // (a ticket each)
+            const uint32_t now = n_seqs - s0 < kVerifyTickets ? n_seqs - s0 : kVerifyTickets;
+            a.seq0 = s0;
+            hipLaunchKernelGGL(verify_kernel, dim3((uint32_t)(now * chunks)), dim3(256), 0, be->stream, a);
+            if ((rc = check_launch("verify_drafts"))) return rc;
+        }
+        return YULE_OK;
     });
 }
