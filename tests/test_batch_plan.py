@@ -49,13 +49,13 @@ int main() {
         const uint32_t kv = 1 + rnd(16), group = 1 + rnd(16), hd = 8 * (1 + rnd(32)), seqs = 1 + rnd(200);
         const uint32_t tokens = 1 + rnd(64), prefix = rnd(3) ? rnd(1u << (1 + rnd(20))) : 0;
         const uint32_t cap = rnd(5) ? rnd(1u << (1 + rnd(14))) : 0;
-        const PrefixPlan p = prefix_plan(prefix, cap, seqs, tokens, kv * group, kv, hd, 256);
+        const PrefixPlan p = prefix_plan(prefix, cap, seqs, tokens, kv * group, kv, hd, 2 + 2 * rnd(2), 256);
         CHECK(p.rows == (uint64_t)seqs * tokens * kv * group);
         CHECK((uint64_t)p.p_chunk * p.n_p >= prefix && (!p.n_p || (uint64_t)p.p_chunk * (p.n_p - 1) < prefix));
         CHECK((uint64_t)p.t_chunk * p.n_t >= cap && (!p.n_t || (uint64_t)p.t_chunk * (p.n_t - 1) < cap));
         CHECK(p.n_p + p.n_t <= kMaxParts);
         CHECK((prefix == 0) == (p.n_p == 0) && (cap == 0) == (p.n_t == 0));
-        CHECK((uint64_t)p.p_tiles * kAttnTileRows >= (uint64_t)seqs * tokens * group);
+        CHECK((uint64_t)p.p_tiles * p.p_slots >= (uint64_t)seqs * tokens * group && p.p_slots % 32 == 0);
         CHECK((uint64_t)p.t_tiles * kAttnTileRows >= (uint64_t)tokens * group);
         CHECK(p.p_jobs == (uint64_t)p.n_p * p.p_tiles * kv && p.t_jobs == (uint64_t)p.n_t * p.t_tiles * kv * seqs);
         if (p.n_p + p.n_t) {

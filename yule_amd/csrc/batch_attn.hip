@@ -110,6 +110,12 @@ __device__ __forceinline__ uint32_t opaque(uint32_t x) {
     return x;
 }
 
+// an address that is the same in every lane, in scalar registers
+__device__ __forceinline__ const uint8_t *uniform(uint64_t x) {
+    return reinterpret_cast<const uint8_t *>((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(x >> 32)) << 32 |
+                                             (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)x));
+}
+
 // rows of a cache or activation: address of row 0 of one head, bytes between rows
 struct Rows {
     const uint8_t *p;
@@ -140,11 +146,32 @@ struct WaveAttn {
         l = 0.f;
     }
 
-    // the subtile's scores into probabilities, sums rescaled where a maximum moved
-    __device__ __forceinline__ void softmax(f16v &s, float c) {
-        float cm = s[0];
+    // S^T = K Q^T with K's subtile at k
+    __device__ __forceinline__ f16v scores(const uint8_t *k, uint32_t lane) const {
+        const uint32_t r = lane & 31u, h = lane >> 5;
+        f16v s;
 #pragma unroll
-        for (int i = 1; i < 16; i++) cm = fmaxf(cm, s[i]);
+        for (int i = 0; i < 16; i++) s[i] = 0.f;
+#pragma unroll
+        for (uint32_t st = 0; st < NS; st++)
+            s = mma16<T>(*reinterpret_cast<const i4v *>(k + r * RB + (((2 * st + h) ^ swizzle<C, 1>(r)) << 4)), q[st], s);
+        return s;
+    }
+    // key0: the subtile's first key; the slot sees keys below lim
+    __device__ __forceinline__ static void hide(f16v &s, uint32_t key0, uint32_t lim, uint32_t lane) {
+#pragma unroll
+        for (int i = 0; i < 16; i++)
+            if (key0 + 8 * (i / 4) + 4 * (lane >> 5) + i % 4 >= lim) s[i] = -INFINITY;
+    }
+
+    // the subtiles' scores into probabilities, sums rescaled where a maximum moved
+    template <uint32_t N>
+    __device__ __forceinline__ void softmax(f16v (&s)[N], float c) {
+        float cm = s[0][0];
+#pragma unroll
+        for (uint32_t n = 0; n < N; n++)
+#pragma unroll
+            for (int i = n ? 0 : 1; i < 16; i++) cm = fmaxf(cm, s[n][i]);
         cm = fmaxf(cm, __shfl_xor(cm, 32, 64)) * c;
         if (__ballot(cm > m)) {
             const float mn = fmaxf(m, cm);
@@ -159,15 +186,17 @@ struct WaveAttn {
         }
         const float mb = m == -INFINITY ? 0.f : m;   // nothing seen yet: weights of 0
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-            s[i] = __builtin_amdgcn_exp2f(fmaf(s[i], c, -mb));
-            l += s[i];
-        }
+        for (uint32_t n = 0; n < N; n++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                s[n][i] = __builtin_amdgcn_exp2f(fmaf(s[n][i], c, -mb));
+                l += s[n][i];
+            }
     }
 
     // O^T += V^T P^T with V's subtile at v
-    __device__ __forceinline__ void values(const f16v &s, const uint8_t *v, uint32_t tid) {
-        const uint32_t lane = opaque(tid) & 63u, h = lane >> 5;
+    __device__ __forceinline__ void values(const f16v &s, const uint8_t *v, uint32_t lane) {
+        const uint32_t h = lane >> 5;
         if constexpr (SZ == 4) {
             const uint32_t d = lane & 31u;
 #pragma unroll
@@ -229,6 +258,14 @@ struct WaveAttn {
         }
     }
 
+    // some element of V's subtile is infinite or NaN (the same in every lane)
+    __device__ __forceinline__ static bool holds_not_finite(const uint8_t *v, uint32_t lane) {
+        bool bad = false;
+#pragma unroll
+        for (uint32_t i = 0; i < NL; i++) bad |= not_finite<T>(*reinterpret_cast<const i4v *>(v + 1024 * i + 16 * lane));
+        return __ballot(bad) != 0;
+    }
+
     // Keys key, key + step, .. < k1 in subtiles of 32 (lds: this wave's K subtile
     // and V subtile).  A slot sees keys below lim; every slot sees those below
     // lim_all.  The next K subtile is on its way while this one's softmax and
@@ -238,7 +275,6 @@ struct WaveAttn {
     __device__ __forceinline__ void walk(const Rows &K, const Rows &V, uint32_t hb, uint32_t key, uint32_t step,
                                          uint32_t k1, uint32_t lim, uint32_t lim_all, uint8_t *lds, uint32_t lane,
                                          float c) {
-        const uint32_t h = lane >> 5;
         const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)reinterpret_cast<uintptr_t>((lds_b)lds));
         uint8_t *const vt = lds + SUB;
         if (hb < RB) {   // chunks past the head stay zero: copies leave them out
@@ -250,10 +286,7 @@ struct WaveAttn {
         // the last key repeat it (hidden, and the number of copies stays).
         auto copy = [&](const Rows &R, auto is_v, uint32_t at) {
             constexpr uint32_t STEP = decltype(is_v)::value ? 2 : 1;
-            const uint64_t row = reinterpret_cast<uint64_t>(R.p) + (uint64_t)at * R.stride;
-            const uint8_t *base = reinterpret_cast<const uint8_t *>(
-                (uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(row >> 32)) << 32 |
-                (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)row));
+            const uint8_t *base = uniform(reinterpret_cast<uint64_t>(R.p) + (uint64_t)at * R.stride);
             const uint32_t last = k1 - at - 1u, ln = opaque(lane) & 63u;
 #pragma unroll
             for (uint32_t i = 0; i < NL; i++) {
@@ -272,37 +305,16 @@ struct WaveAttn {
         for (; key < k1; key += step) {
             const bool more = key + step < k1;
             wait_copies<NL>();   // K is there
-            f16v s;
-#pragma unroll
-            for (int i = 0; i < 16; i++) s[i] = 0.f;
-            {
-                const uint32_t ln = opaque(lane) & 63u, r = ln & 31u, hh = ln >> 5;
-#pragma unroll
-                for (uint32_t st = 0; st < NS; st++) {
-                    const i4v a = *reinterpret_cast<const i4v *>(lds + r * RB + (((2 * st + hh) ^ swizzle<C, 1>(r)) << 4));
-                    s = mma16<T>(a, q[st], s);
-                }
-            }
+            f16v s[1] = {scores(lds, opaque(lane) & 63u)};
             wait_lds();
             if (more) copy(K, No{}, key + step);
             const bool masked = key + 32 > lim_all;
-            if (masked) {
-#pragma unroll
-                for (int i = 0; i < 16; i++)
-                    if (key + 8 * (i / 4) + 4 * h + i % 4 >= lim) s[i] = -INFINITY;
-            }
+            if (masked) hide(s[0], key, lim, lane);
             softmax(s, c);
             if (more) wait_copies<NL>();   // V is there
             else wait_copies<0>();
-            bool odd = false;
-            if (masked) {
-#pragma unroll
-                for (uint32_t i = 0; i < NL; i++)
-                    odd |= not_finite<T>(*reinterpret_cast<const i4v *>(vt + 1024 * i + 16 * lane));
-                odd = __ballot(odd) != 0;
-            }
-            if (odd) values_seen(s, vt, lane, key, lim);
-            else values(s, vt, lane);
+            if (masked && holds_not_finite(vt, lane)) values_seen(s[0], vt, lane, key, lim);
+            else values(s[0], vt, opaque(lane) & 63u);
             wait_lds();
             if (more) copy(V, Yes{}, key + step);
         }
@@ -367,6 +379,112 @@ struct BlockAttn {
     }
 };
 
+// ---- a workgroup of four waves with 32 slots each over tiles of keys that they
+// share (16-bit types): tiles of NSUB subtiles, the next one's K and V on their
+// way into the other half of the LDS while this one is worked on.
+template <typename T, uint32_t D>
+struct TileAttn {
+    using W = WaveAttn<T, D>;
+    static constexpr uint32_t NW = 4, NSUB = W::SUB <= 8192 ? 2 : 1, TILE = NSUB * W::SUB, KEYS = 32 * NSUB;
+    static constexpr uint32_t NC = NSUB * W::NL / NW;   // copies of a wave per tile of K, and of V
+    static_assert(NSUB * W::NL % NW == 0);
+    struct Shared {
+        __align__(1024) uint8_t kv[2][2][TILE];
+    };
+
+    // Every wave: its slots' keys below k1 (the workgroup's); the wave's slots see
+    // keys below lim (each lane's own), all of them those below lim_lo, none those
+    // from lim_hi (0: the wave has no slots).  out(dim, four sums, maximum, weight) of the lane's slot.
+    template <typename OUT>
+    __device__ __forceinline__ static void run(Shared &sh, const uint8_t *qrow, const Rows &K, const Rows &V, uint32_t hb,
+                                               uint32_t k0, uint32_t k1, uint32_t lim, uint32_t lim_lo, uint32_t lim_hi,
+                                               float c, OUT out) {
+        constexpr uint32_t RB = W::RB, C = W::C, SUB = W::SUB;
+        const uint32_t tid = threadIdx.x, lane = tid & 63u, h = lane >> 5;
+        const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>((lds_b)&sh.kv[0][0][0]) + 1024 * NC * wave;
+        W w;
+        w.init(qrow, hb, h);
+        if (hb < RB) {   // chunks past the head stay zero: copies leave them out
+            for (uint32_t i = tid; i < 4 * TILE / 16; i += 64 * NW) *reinterpret_cast<i4v *>(&sh.kv[0][0][0] + 16 * i) = i4v{0, 0, 0, 0};
+            wait_lds();
+            __builtin_amdgcn_s_barrier();
+        }
+        // this lane's part of its wave's copies: LDS chunk 64 (NC wave + i) + lane of the tile
+        uint32_t off[2][NC];
+#pragma unroll
+        for (uint32_t i = 0; i < NC; i++) {
+            const uint32_t L = 64 * (NC * wave + i) + lane, r = L / C;
+            const uint32_t kc = 16 * ((L % C) ^ swizzle<C, 1>(r)), vc = 16 * ((L % C) ^ swizzle<C, 2>(r));
+            off[0][i] = kc < hb ? r * K.stride + kc : ~0u;
+            off[1][i] = vc < hb ? r * V.stride + vc : ~0u;
+        }
+        auto copy = [&](uint32_t at, uint32_t buf) {
+            const uint64_t kr = reinterpret_cast<uint64_t>(K.p) + (uint64_t)at * K.stride;
+            const uint64_t vr = reinterpret_cast<uint64_t>(V.p) + (uint64_t)at * V.stride;
+            const uint8_t *kb = uniform(kr), *vb = uniform(vr);
+            const uint32_t dst = lds0 + 2 * TILE * buf;
+            if (k1 - at >= KEYS && hb == RB) {
+#pragma unroll
+                for (uint32_t i = 0; i < NC; i++) copy_to_lds(kb, off[0][i], dst + 1024 * i);
+#pragma unroll
+                for (uint32_t i = 0; i < NC; i++) copy_to_lds(vb, off[1][i], dst + TILE + 1024 * i);
+            } else if (k1 - at >= KEYS) {
+#pragma unroll
+                for (uint32_t i = 0; i < NC; i++)
+                    if (off[0][i] != ~0u) copy_to_lds(kb, off[0][i], dst + 1024 * i);
+#pragma unroll
+                for (uint32_t i = 0; i < NC; i++)
+                    if (off[1][i] != ~0u) copy_to_lds(vb, off[1][i], dst + TILE + 1024 * i);
+            } else {   // rows past the last key repeat it (hidden)
+                const uint32_t last = k1 - at - 1u;
+#pragma unroll
+                for (uint32_t i = 0; i < NC; i++) {
+                    const uint32_t L = 64 * (NC * wave + i) + (opaque(lane) & 63u), r = L / C, rr = r < last ? r : last;
+                    const uint32_t kc = 16 * ((L % C) ^ swizzle<C, 1>(r)), vc = 16 * ((L % C) ^ swizzle<C, 2>(r));
+                    if (kc < hb) copy_to_lds(kb, rr * K.stride + kc, dst + 1024 * i);
+                    if (vc < hb) copy_to_lds(vb, rr * V.stride + vc, dst + TILE + 1024 * i);
+                }
+            }
+        };
+        copy(k0, 0);
+        uint32_t buf = 0;
+        for (uint32_t key = k0; key < k1; key += KEYS, buf ^= 1u) {
+            wait_copies<0>();
+            wait_lds();
+            __builtin_amdgcn_s_barrier();   // every wave's copies are there, and nobody reads the other half
+            __atomic_signal_fence(__ATOMIC_SEQ_CST);
+            if (key + KEYS < k1) copy(key + KEYS, buf ^ 1u);
+            const uint8_t *kt = &sh.kv[buf][0][0], *vt = &sh.kv[buf][1][0];
+            if (key + KEYS <= lim_lo) {
+                f16v s[NSUB];
+#pragma unroll
+                for (uint32_t n = 0; n < NSUB; n++) s[n] = w.scores(kt + n * SUB, lane);
+                w.softmax(s, c);
+#pragma unroll
+                for (uint32_t n = 0; n < NSUB; n++) w.values(s[n], vt + n * SUB, lane);
+            } else {
+#pragma unroll 1
+                for (uint32_t n = 0; n < NSUB; n++) {
+                    const uint32_t key0 = key + 32 * n;
+                    if (key0 >= lim_hi) break;
+                    f16v s[1] = {w.scores(kt + n * SUB, lane)};
+                    W::hide(s[0], key0, lim, lane);
+                    w.softmax(s, c);
+                    if (W::holds_not_finite(vt + n * SUB, lane)) w.values_seen(s[0], vt + n * SUB, lane, key0, lim);
+                    else w.values(s[0], vt + n * SUB, opaque(lane) & 63u);
+                }
+            }
+        }
+        const float l = w.l + __shfl_xor(w.l, 32, 64);
+#pragma unroll
+        for (uint32_t t = 0; t < W::DT; t++)
+#pragma unroll
+            for (uint32_t a = 0; a < 4; a++)
+                out(32 * t + 8 * a + 4 * h, f4v{w.o[t][4 * a], w.o[t][4 * a + 1], w.o[t][4 * a + 2], w.o[t][4 * a + 3]}, w.m, l);
+    }
+};
+
 // four results of a row, rounded once to its type
 template <typename T>
 __device__ __forceinline__ void store4(uint8_t *row, uint32_t d, f4v x) {
@@ -397,6 +515,7 @@ struct PromptArgs {
 // inside it (tiles of a sequence from the last, with the most keys, to the
 // first).  Offsets are the caller's data on the device: rows are clamped to the
 // buffers'.  False past the last tile.
+template <uint32_t SLOTS>
 __device__ __forceinline__ bool find_tile(const uint32_t *off, uint32_t n_seqs, uint32_t n_rows, uint32_t group,
                                           uint32_t y, uint32_t lane, uint32_t *row0, uint32_t *len, uint32_t *tile) {
     uint32_t before = 0;
@@ -410,7 +529,7 @@ __device__ __forceinline__ bool find_tile(const uint32_t *off, uint32_t n_seqs, 
             e = e < n_rows ? e : n_rows;
             e = e > b ? e : b;
         }
-        const uint32_t mine = ((e - b) * group + kAttnTileRows - 1) / kAttnTileRows;
+        const uint32_t mine = ((e - b) * group + SLOTS - 1) / SLOTS;
         uint32_t sum = mine;
 #pragma unroll
         for (uint32_t d = 1; d < 64; d *= 2) {
@@ -437,7 +556,7 @@ __global__ __launch_bounds__((64 * BlockAttn<T, D>::NW))
     __shared__ typename B::Shared sh;
     const uint32_t kvh = blockIdx.x % a.s.n_kv, lane = threadIdx.x & 63u;
     uint32_t row0, len, tile;
-    if (!find_tile(a.off, a.n_seqs, a.n_rows, a.s.group, blockIdx.x / a.s.n_kv, lane, &row0, &len, &tile)) return;
+    if (!find_tile<kAttnTileRows>(a.off, a.n_seqs, a.n_rows, a.s.group, blockIdx.x / a.s.n_kv, lane, &row0, &len, &tile)) return;
     const uint32_t slots = len * a.s.group, slot0 = tile * kAttnTileRows, hb = a.s.hd * sizeof(T);
     const uint32_t last = (slot0 + kAttnTileRows < slots ? slot0 + kAttnTileRows : slots) - 1u;
     auto at = [&](uint32_t slot, uint32_t stride) {   // the slot's bytes in q or out
@@ -452,78 +571,111 @@ __global__ __launch_bounds__((64 * BlockAttn<T, D>::NW))
            });
 }
 
+// the same by workgroups of 128 slots
+template <typename T, uint32_t D>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void prompt_tile_kernel(PromptArgs a) {
+    using B = TileAttn<T, D>;
+    __shared__ typename B::Shared sh;
+    const uint32_t kvh = blockIdx.x % a.s.n_kv, lane = threadIdx.x & 63u, g = a.s.group;
+    uint32_t row0, len, tile;
+    if (!find_tile<128>(a.off, a.n_seqs, a.n_rows, g, blockIdx.x / a.s.n_kv, lane, &row0, &len, &tile)) return;
+    const uint32_t hb = a.s.hd * sizeof(T), end = len * g - 1u, slot0 = 128 * tile;
+    const uint32_t last = slot0 + 127 < end ? slot0 + 127 : end;   // the workgroup's last slot
+    const uint32_t first_w = slot0 + 32 * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t last_w = first_w + 31 < last ? first_w + 31 : last, mine = first_w + (lane & 31u) < last ? first_w + (lane & 31u) : last;
+    const uint32_t r = mine / g;
+    const size_t head = (size_t)(kvh * g + (mine - r * g)) * hb;
+    const Rows K = {a.k + (size_t)row0 * a.ks + (size_t)kvh * hb, a.ks}, V = {a.v + (size_t)row0 * a.vs + (size_t)kvh * hb, a.vs};
+    const bool any = first_w <= last, own = first_w + (lane & 31u) <= last;
+    uint8_t *const out = a.out + (size_t)(row0 + r) * a.os + head;
+    B::run(sh, a.q + (size_t)(row0 + r) * a.qs + head, K, V, hb, 0, last / g + 1u, r + 1u, any ? first_w / g + 1u : 0u,
+           any ? last_w / g + 1u : 0u, a.s.c, [&](uint32_t d, f4v o, float, float L) {
+               if (own && d < a.s.hd) store4<T>(out, d, o * (L == 0.f ? 0.f : 1.0f / L));
+           });
+}
+
 // ---- new tokens over a shared prefix and their own tails
 struct PrefixArgs {
     const uint8_t *q, *kp, *vp, *kt, *vt;
     uint32_t qs, kps, vps, kts, vts;
     const uint32_t *lens;
     uint32_t prefix, cap, n_seqs, n_tokens;
-    uint32_t p_chunk, n_p, p_tiles, t_chunk, n_t, t_tiles, p_jobs;
+    uint32_t p_chunk, n_p, p_tiles, t_chunk, n_t, t_tiles, p_jobs;   // (p_jobs: of one KV head)
     float2 *ml;   // [chunk][row][head]
     float *o;     // [chunk][row][head][hd]
     HeadShape s;
 };
 
-template <typename T, uint32_t D>
+// TILE: the prefix by workgroups of 128 slots that share its tiles
+template <typename T, uint32_t D, bool TILE>
 __global__ __launch_bounds__((64 * BlockAttn<T, D>::NW))
     __attribute__((amdgpu_waves_per_eu(BlockAttn<T, D>::WAVES))) void prefix_attn_kernel(PrefixArgs a) {
     using B = BlockAttn<T, D>;
-    __shared__ typename B::Shared sh;
+    using P = TileAttn<T, D>;
+    __shared__ union {
+        typename B::Shared block;
+        typename std::conditional<TILE, typename P::Shared, char>::type tile;
+    } sh;
     const uint32_t lane = threadIdx.x & 63u, hb = a.s.hd * sizeof(T), g = a.s.group, n_heads = g * a.s.n_kv;
-    uint32_t job = blockIdx.x, row0, slots, tile, chunk, k0, k1, lim, lim_all;
-    const uint32_t kvh = job % a.s.n_kv;
-    Rows K, V;
-    uint32_t last, slot0, mine;
-    auto place = [&]() {
-        slot0 = tile * kAttnTileRows;
-        last = (slot0 + kAttnTileRows < slots ? slot0 + kAttnTileRows : slots) - 1u;
-        mine = slot0 + (lane & 31u) < last ? slot0 + (lane & 31u) : last;
-    };
-    if (job < a.p_jobs) {
-        job /= a.s.n_kv;
-        tile = job % a.p_tiles;
-        chunk = job / a.p_tiles;
-        row0 = 0;
-        slots = a.n_seqs * a.n_tokens * g;
-        place();
-        k0 = chunk * a.p_chunk;
-        k1 = a.prefix - k0 < a.p_chunk ? a.prefix : k0 + a.p_chunk;
-        lim = lim_all = k1;
-        K = {a.kp + (size_t)kvh * hb, a.kps};
-        V = {a.vp + (size_t)kvh * hb, a.vps};
-    } else {
-        job = (job - a.p_jobs) / a.s.n_kv;
-        tile = job % a.t_tiles;
-        job /= a.t_tiles;
-        const uint32_t seq = job % a.n_seqs, len = a.lens[seq] < a.cap ? a.lens[seq] : a.cap;
-        chunk = job / a.n_seqs;
-        row0 = seq * a.n_tokens;
-        slots = a.n_tokens * g;
-        place();
-        // token i sees rows below len - n_tokens + 1 + i of the tail
-        auto sees = [&](uint32_t slot) {
-            const uint32_t n = len + 1u + slot / g;
-            return n > a.n_tokens ? n - a.n_tokens : 0u;
-        };
-        k0 = chunk * a.t_chunk;
-        k1 = sees(last) < k0 + a.t_chunk ? sees(last) : k0 + a.t_chunk;
-        lim = sees(mine) < k1 ? sees(mine) : k1;
-        lim_all = sees(slot0);
-        K = {a.kt + (size_t)seq * a.cap * a.kts + (size_t)kvh * hb, a.kts};
-        V = {a.vt + (size_t)seq * a.cap * a.vts + (size_t)kvh * hb, a.vts};
-        chunk += a.n_p;
-    }
+    const uint32_t kvh = blockIdx.x % a.s.n_kv, n_rows = a.n_seqs * a.n_tokens;
+    uint32_t job = blockIdx.x / a.s.n_kv, row0 = 0;
     auto pair = [&](uint32_t slot) {   // (row, head) of the slot
         const uint32_t r = slot / g;
         return (size_t)(row0 + r) * n_heads + kvh * g + (slot - r * g);
     };
-    const size_t part = (size_t)chunk * a.n_seqs * a.n_tokens * n_heads;
+    auto query = [&](uint32_t slot) {
+        const uint32_t r = slot / g;
+        return a.q + (size_t)(row0 + r) * a.qs + (size_t)(kvh * g + (slot - r * g)) * hb;
+    };
+    if (job < a.p_jobs) {
+        const uint32_t tile = job % a.p_tiles, chunk = job / a.p_tiles, slots = n_rows * g;
+        const uint32_t k0 = chunk * a.p_chunk, k1 = a.prefix - k0 < a.p_chunk ? a.prefix : k0 + a.p_chunk;
+        const Rows K = {a.kp + (size_t)kvh * hb, a.kps}, V = {a.vp + (size_t)kvh * hb, a.vps};
+        const size_t part = (size_t)chunk * n_rows * n_heads;
+        if constexpr (TILE) {
+            const uint32_t first = 128 * tile + 32 * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), slot = first + (lane & 31u);
+            const uint32_t mine = slot < slots ? slot : slots - 1u;
+            const size_t at = part + pair(mine);
+            P::run(sh.tile, query(mine), K, V, hb, k0, k1, k1, first < slots ? k1 : 0u, first < slots ? k1 : 0u, a.s.c,
+                   [&](uint32_t d, f4v o, float M, float L) {
+                       if (slot >= slots || d >= a.s.hd) return;
+                       if (d == 0) a.ml[at] = make_float2(M, L);
+                       *reinterpret_cast<f4v *>(a.o + at * a.s.hd + d) = o;
+                   });
+        } else {
+            const uint32_t slot0 = tile * kAttnTileRows, slot = slot0 + (lane & 31u);
+            B::run(sh.block, query(slot < slots ? slot : slots - 1u), K, V, hb, k0, k1, k1, k1, a.s.c,
+                   [&](uint32_t i, uint32_t d, f4v o, float M, float L) {
+                       if (slot0 + i >= slots || d >= a.s.hd) return;
+                       const size_t at = part + pair(slot0 + i);
+                       if (d == 0) a.ml[at] = make_float2(M, L);
+                       *reinterpret_cast<f4v *>(a.o + at * a.s.hd + d) = o;
+                   });
+        }
+        return;
+    }
+    job -= a.p_jobs;
+    const uint32_t tile = job % a.t_tiles;
+    job /= a.t_tiles;
+    const uint32_t seq = job % a.n_seqs, len = a.lens[seq] < a.cap ? a.lens[seq] : a.cap, chunk = job / a.n_seqs;
+    row0 = seq * a.n_tokens;
+    const uint32_t slots = a.n_tokens * g, slot0 = tile * kAttnTileRows;
+    const uint32_t last = slot0 + kAttnTileRows < slots ? slot0 + kAttnTileRows - 1u : slots - 1u;
+    const uint32_t mine = slot0 + (lane & 31u) < last ? slot0 + (lane & 31u) : last;
+    // token i sees rows below len - n_tokens + 1 + i of the tail
+    auto sees = [&](uint32_t slot) {
+        const uint32_t n = len + 1u + slot / g;
+        return n > a.n_tokens ? n - a.n_tokens : 0u;
+    };
+    const uint32_t k0 = chunk * a.t_chunk, k1 = sees(last) < k0 + a.t_chunk ? sees(last) : k0 + a.t_chunk;
+    const size_t part = (size_t)(a.n_p + chunk) * n_rows * n_heads;
     if (k0 >= k1) {   // nothing of the tail in this chunk
         if (threadIdx.x < 32 && slot0 + threadIdx.x <= last) a.ml[part + pair(slot0 + threadIdx.x)] = make_float2(-INFINITY, 0.f);
         return;
     }
-    const uint32_t r = mine / g;
-    B::run(sh, a.q + (size_t)(row0 + r) * a.qs + (size_t)(kvh * g + (mine - r * g)) * hb, K, V, hb, k0, k1, lim, lim_all, a.s.c,
+    const Rows K = {a.kt + (size_t)seq * a.cap * a.kts + (size_t)kvh * hb, a.kts};
+    const Rows V = {a.vt + (size_t)seq * a.cap * a.vts + (size_t)kvh * hb, a.vts};
+    B::run(sh.block, query(mine), K, V, hb, k0, k1, sees(mine) < k1 ? sees(mine) : k1, sees(slot0), a.s.c,
            [&](uint32_t i, uint32_t d, f4v o, float M, float L) {
                if (slot0 + i > last || d >= a.s.hd) return;
                const size_t at = part + pair(slot0 + i);
@@ -612,20 +764,33 @@ static HeadShape head_shape(uint32_t n_heads, uint32_t n_kv, uint32_t hd) {
     return {n_heads / n_kv, n_kv, hd, (float)(1.44269504088896340736 / sqrt((double)hd))};
 }
 
-static int launch_prompt(hipStream_t s, const PromptArgs &a, uint32_t dtype, uint64_t workgroups) {
+static int launch_prompt(hipStream_t s, const PromptArgs &a, uint32_t dtype, uint64_t tiles, bool shared) {
+    const dim3 grid((uint32_t)(tiles * a.s.n_kv));
     by_shape(dtype, a.s.hd, [&](auto t, auto d) {
         using T = decltype(t);
         constexpr uint32_t D = decltype(d)::value;
-        hipLaunchKernelGGL((prompt_attn_kernel<T, D>), dim3((uint32_t)workgroups), dim3(64 * BlockAttn<T, D>::NW), 0, s, a);
+        if constexpr (sizeof(T) == 2) {
+            if (shared) {
+                hipLaunchKernelGGL((prompt_tile_kernel<T, D>), grid, dim3(256), 0, s, a);
+                return;
+            }
+        }
+        hipLaunchKernelGGL((prompt_attn_kernel<T, D>), grid, dim3(64 * BlockAttn<T, D>::NW), 0, s, a);
     });
     return check_launch("prompt_attn");
 }
 
-static int launch_prefix(hipStream_t s, const PrefixArgs &a, uint32_t dtype, uint64_t workgroups) {
+static int launch_prefix(hipStream_t s, const PrefixArgs &a, uint32_t dtype, uint64_t workgroups, bool tile) {
     by_shape(dtype, a.s.hd, [&](auto t, auto d) {
         using T = decltype(t);
         constexpr uint32_t D = decltype(d)::value;
-        hipLaunchKernelGGL((prefix_attn_kernel<T, D>), dim3((uint32_t)workgroups), dim3(64 * BlockAttn<T, D>::NW), 0, s, a);
+        if constexpr (sizeof(T) == 2) {
+            if (tile) {
+                hipLaunchKernelGGL((prefix_attn_kernel<T, D, true>), dim3((uint32_t)workgroups), dim3(256), 0, s, a);
+                return;
+            }
+        }
+        hipLaunchKernelGGL((prefix_attn_kernel<T, D, false>), dim3((uint32_t)workgroups), dim3(64 * BlockAttn<T, D>::NW), 0, s, a);
     });
     return check_launch("prefix_attn");
 }
@@ -691,12 +856,15 @@ int yule_hip_prompt_attn(yule_hip_backend *be, const yule_rows *q, const yule_ro
             return set_error(YULE_ERR_INVALID, "prompt_attn: an input and the output alias");
         if (!n_seqs || !n_rows) return YULE_OK;
         // tiles of all sequences: each has at most one that is not full
-        const uint64_t group = n_heads / n_kv_heads, tiles = n_rows * group / kAttnTileRows + n_seqs;
+        const uint64_t group = n_heads / n_kv_heads;
+        const char *force = getenv("YULE_PROMPT_TILE");
+        const bool shared = elem == 2 && (force ? atoi(force) != 0 : true);
+        const uint64_t tiles = n_rows * group / (shared ? 128 : kAttnTileRows) + n_seqs;
         if ((uint64_t)n_rows * group >= (uint64_t)1 << 31 || tiles * n_kv_heads > kMaxWorkgroups)
             return set_error(YULE_ERR_INVALID, "prompt_attn: too many rows for one call");
         const PromptArgs a = {cq.p, ck.p, cv.p, co.p, cq.stride, ck.stride, cv.stride, co.stride,
                               static_cast<const uint32_t *>(off), n_seqs, n_rows, head_shape(n_heads, n_kv_heads, head_dim)};
-        return launch_prompt(be->stream, a, dtype, tiles * n_kv_heads);
+        return launch_prompt(be->stream, a, dtype, tiles, shared);
     });
 }
 
@@ -730,7 +898,7 @@ int yule_hip_prefix_attn(yule_hip_backend *be, const yule_rows *q, const yule_ro
             (tail_cap && (out->buffer == k_tail->buffer || out->buffer == v_tail->buffer)))
             return set_error(YULE_ERR_INVALID, "prefix_attn: an input and the output alias");
         if (!n_seqs) return YULE_OK;
-        const PrefixPlan p = prefix_plan(prefix_len, tail_cap, n_seqs, n_tokens, n_heads, n_kv_heads, head_dim,
+        const PrefixPlan p = prefix_plan(prefix_len, tail_cap, n_seqs, n_tokens, n_heads, n_kv_heads, head_dim, elem,
                                          (uint32_t)be->props.multiProcessorCount);
         if (p.rows > kMaxWorkgroups || p.p_jobs + p.t_jobs > kMaxWorkgroups)
             return set_error(YULE_ERR_INVALID, "prefix_attn: too many rows for one call");
@@ -742,11 +910,11 @@ int yule_hip_prefix_attn(yule_hip_backend *be, const yule_rows *q, const yule_ro
         a.lens = static_cast<const uint32_t *>(lens);
         a.prefix = prefix_len, a.cap = tail_cap, a.n_seqs = n_seqs, a.n_tokens = n_tokens;
         a.p_chunk = p.p_chunk, a.n_p = p.n_p, a.p_tiles = p.p_tiles;
-        a.t_chunk = p.t_chunk, a.n_t = p.n_t, a.t_tiles = p.t_tiles, a.p_jobs = (uint32_t)p.p_jobs;
+        a.t_chunk = p.t_chunk, a.n_t = p.n_t, a.t_tiles = p.t_tiles, a.p_jobs = (uint32_t)(p.p_jobs / n_kv_heads);
         a.ml = static_cast<float2 *>(ws.ptr);
         a.o = reinterpret_cast<float *>(static_cast<uint8_t *>(ws.ptr) + p.ml_bytes);
         a.s = head_shape(n_heads, n_kv_heads, head_dim);
-        if (p.p_jobs + p.t_jobs && (rc = launch_prefix(be->stream, a, dtype, p.p_jobs + p.t_jobs))) return rc;
+        if (p.p_jobs + p.t_jobs && (rc = launch_prefix(be->stream, a, dtype, p.p_jobs + p.t_jobs, p.p_slots > kAttnTileRows))) return rc;
         return launch_join(be->stream, a, co.p, co.stride, dtype);
     });
 }

@@ -50,13 +50,13 @@ constexpr uint32_t kAttnTileRows = 32;
 constexpr uint64_t kMaxWorkgroups = (uint64_t)1 << 23;
 constexpr uint32_t kMaxKeys = 1u << 30;   // of a prefix, and of a tail
 
-// ---- verify_drafts: values of a row per workgroup, and what a chunk leaves
-// (f64 sums of max(p - q, 0) and of p, and the last places where they are not 0)
+// ---- verify_drafts: values of a row per workgroup, and what a chunk leaves (the
+// f64 sum of its weights, and the last place that has one)
 constexpr uint32_t kVerifyChunk = 4096, kMaxVocab = 1u << 30, kMaxDrafts = 1024;
 constexpr uint32_t kVerifyTickets = 4096;   // sequences of one launch
 struct VerifySum {
-    double rest, whole;
-    int last_rest, last_whole;
+    double sum;
+    int64_t last;
 };
 
 // chunks of a prefix and a tail together
@@ -68,6 +68,7 @@ constexpr uint32_t kMaxParts = 1024;
 struct PrefixPlan {
     uint32_t p_chunk, n_p;   // keys of a prefix chunk, chunks (0 without a prefix)
     uint32_t t_chunk, n_t;   // the same of a tail
+    uint32_t p_slots;            // (query row, head of the group) pairs of a prefix tile
     uint32_t p_tiles, t_tiles;   // query tiles per KV head over the whole batch, and per sequence
     uint64_t rows;           // (query row, head) pairs
     uint64_t p_jobs, t_jobs;
@@ -79,10 +80,11 @@ struct PrefixPlan {
 };
 
 inline PrefixPlan prefix_plan(uint32_t prefix_len, uint32_t tail_cap, uint32_t n_seqs, uint32_t n_tokens,
-                              uint32_t n_heads, uint32_t n_kv, uint32_t hd, uint32_t cus) {
+                              uint32_t n_heads, uint32_t n_kv, uint32_t hd, uint32_t elem, uint32_t cus) {
     PrefixPlan p{};
     const uint64_t group = n_heads / n_kv, slots = (uint64_t)n_seqs * n_tokens * group;
-    p.p_tiles = (uint32_t)((slots + kAttnTileRows - 1) / kAttnTileRows);
+    p.p_slots = elem == 2 && slots > kAttnTileRows ? 128u : kAttnTileRows;
+    p.p_tiles = (uint32_t)((slots + p.p_slots - 1) / p.p_slots);
     p.t_tiles = (uint32_t)((n_tokens * group + kAttnTileRows - 1) / kAttnTileRows);
     // enough chunks for two workgroups a CU, none below 256 keys (two tiles of every wave)
     auto split = [&](uint32_t keys, uint64_t per_chunk, uint32_t *chunk, uint32_t *n) {

@@ -13,7 +13,7 @@
 // One launch: the rows are cut into chunks of 4096 values, a workgroup each,
 // which leave their sums; the workgroup that takes a sequence's last ticket finds
 // the chunk that the pick falls into and walks that one again.
-#include <cmath>
+#include <type_traits>
 
 #include "batch_plan.h"
 #include "internal.h"
@@ -37,23 +37,20 @@ __device__ __forceinline__ double weight(double x) { return x > 0.0 ? x : 0.0; }
 
 // kept drafts of sequence s (the same in every lane of every wave that asks)
 __device__ __forceinline__ uint32_t kept(const VerifyArgs &a, uint32_t s, uint32_t lane, uint32_t *count) {
+    // (what does not depend on another load is loaded first)
     uint32_t n = a.lens ? a.lens[s] : a.n_draft;
-    n = n < a.n_draft ? n : a.n_draft;
-    *count = n;
-    for (uint32_t i0 = 0; i0 < n; i0 += 64) {
-        const uint32_t i = i0 + lane;
-        bool stop = i >= n;
-        if (!stop) {
-            const uint32_t x = a.drafts[(size_t)s * a.n_draft + i];
-            if (x < a.vocab) {
-                const double u = a.u[(size_t)s * (a.n_draft + 1) + i];
-                const double q = a.q[((size_t)s * a.n_draft + i) * a.qs + x];
-                stop = !(u * q < (double)a.p[((size_t)s * (a.n_draft + 1) + i) * a.ps + x]);
-            } else {
-                stop = true;   // not a token: no probability
-            }
-        }
-        const uint64_t stops = __ballot(stop);
+    *count = 0;
+    if (!a.n_draft) return 0;
+    for (uint32_t i0 = 0; i0 < a.n_draft; i0 += 64) {
+        const uint32_t i = i0 + lane < a.n_draft ? i0 + lane : a.n_draft - 1u;
+        const uint32_t x = a.drafts[(size_t)s * a.n_draft + i], xc = x < a.vocab ? x : 0u;
+        const double u = a.u[(size_t)s * (a.n_draft + 1) + i];
+        const double q = a.q[((size_t)s * a.n_draft + i) * a.qs + xc];
+        const double p = a.p[((size_t)s * (a.n_draft + 1) + i) * a.ps + xc];
+        n = n < a.n_draft ? n : a.n_draft;
+        *count = n;
+        // (x of vocab or more is no token and has no probability)
+        const uint64_t stops = __ballot(i0 + lane >= n || x >= a.vocab || !(u * q < p));
         if (stops) return i0 + (uint32_t)__builtin_ctzll(stops);
     }
     return n;
@@ -66,10 +63,28 @@ __device__ __forceinline__ void rows_of(const VerifyArgs &a, uint32_t s, uint32_
     *q = kept < count ? a.q + ((size_t)s * a.n_draft + kept) * a.qs : nullptr;
 }
 
-__device__ __forceinline__ double wave_sum(double x) {
-#pragma unroll
-    for (int d = 32; d; d /= 2) x += __shfl_xor(x, d, 64);
+// inclusive sums over the wave's lanes, by DPP row shifts and row broadcasts
+__device__ __forceinline__ double wave_scan(double x) {
+    auto step = [&](auto ctrl, auto rows) {   // lanes without a source add 0
+        constexpr int CTRL = decltype(ctrl)::value, ROWS = decltype(rows)::value;
+        const uint64_t b = __builtin_bit_cast(uint64_t, x);
+        const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, 0xf, false);
+        const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, ROWS, 0xf, false);
+        x += __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+    };
+    using std::integral_constant;
+    step(integral_constant<int, 0x111>{}, integral_constant<int, 0xf>{});   // row_shr 1, 2, 4, 8
+    step(integral_constant<int, 0x112>{}, integral_constant<int, 0xf>{});
+    step(integral_constant<int, 0x114>{}, integral_constant<int, 0xf>{});
+    step(integral_constant<int, 0x118>{}, integral_constant<int, 0xf>{});
+    step(integral_constant<int, 0x142>{}, integral_constant<int, 0xa>{});   // row_bcast 15, 31
+    step(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});
     return x;
+}
+__device__ __forceinline__ double last_lane(double x) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    return __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(b >> 32), 63) << 32 |
+                                          (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, 63));
 }
 __device__ __forceinline__ int wave_max(int x) {
 #pragma unroll
@@ -102,23 +117,13 @@ __device__ __forceinline__ void load_chunk(const float *row, uint32_t x0, uint32
     }
 }
 
-// inclusive sums over the wave's lanes
-__device__ __forceinline__ double wave_scan(double x, uint32_t lane) {
-#pragma unroll
-    for (uint32_t d = 1; d < 64; d *= 2) {
-        const double y = __shfl_up(x, d, 64);
-        if (lane >= d) x += y;
-    }
-    return x;
-}
-
 // A workgroup per chunk; the one that takes its sequence's last ticket picks and
 // answers.  Sums are taken in one order, whoever is last.
 __global__ __launch_bounds__(256) void verify_kernel(VerifyArgs a) {
-    __shared__ double part[2][16];   // sums of max(p - q, 0), of p, of 256 values each: 1024 j + 256 wave ..
-    __shared__ int lasts[2][4];      // last places where they are not 0, by wave
+    __shared__ double part[16];   // sums of 256 weights each: 1024 j + 256 wave ..
+    __shared__ int lasts[4];      // last places that have a weight, by wave
     __shared__ double target, before;
-    __shared__ uint32_t is_last, at, of_rest, token;
+    __shared__ uint32_t is_last, at, token, again;
     const uint32_t s = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks, seq = a.seq0 + s;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
     uint32_t count;
@@ -126,61 +131,53 @@ __global__ __launch_bounds__(256) void verify_kernel(VerifyArgs a) {
     const float *p, *q;
     rows_of(a, seq, n, count, &p, &q);
 
-    double r[4][4], w[4][4];   // this thread's weights of a chunk
-    auto weigh = [&](uint32_t x0) {
+    double w[4][4];   // this thread's weights of a chunk
+    auto weigh = [&](uint32_t c) {
         float pv[4][4], qv[4][4];
-        load_chunk(p, x0, a.vocab, tid, pv);
-        if (q) load_chunk(q, x0, a.vocab, tid, qv);
+        load_chunk(p, c * kVerifyChunk, a.vocab, tid, pv);
+        if (q) load_chunk(q, c * kVerifyChunk, a.vocab, tid, qv);
 #pragma unroll
         for (uint32_t j = 0; j < 4; j++) {
 #pragma unroll
-            for (uint32_t e = 0; e < 4; e++) {
-                w[j][e] = weight(pv[j][e]);
-                r[j][e] = q ? weight((double)pv[j][e] - (double)qv[j][e]) : w[j][e];
-            }
-            const double sr = wave_sum((r[j][0] + r[j][1]) + (r[j][2] + r[j][3]));
-            const double sw = q ? wave_sum((w[j][0] + w[j][1]) + (w[j][2] + w[j][3])) : sr;
-            if (lane == 0) part[0][4 * j + wave] = sr, part[1][4 * j + wave] = sw;
+            for (uint32_t e = 0; e < 4; e++) w[j][e] = weight(q ? (double)pv[j][e] - (double)qv[j][e] : (double)pv[j][e]);
+            const double sum = last_lane(wave_scan((w[j][0] + w[j][1]) + (w[j][2] + w[j][3])));
+            if (lane == 0) part[4 * j + wave] = sum;
         }
+        int last = -1;
+#pragma unroll
+        for (uint32_t j = 0; j < 4; j++)
+#pragma unroll
+            for (uint32_t e = 0; e < 4; e++)
+                if (w[j][e] > 0.0) last = (int)(c * kVerifyChunk + 1024 * j + 4 * tid + e);
+        last = wave_max(last);
+        if (lane == 0) lasts[wave] = last;
+        __syncthreads();
     };
-    weigh(chunk * kVerifyChunk);
-    int last_r = -1, last_w = -1;
+    // (every thread) the chunk that was weighed
+    auto chunk_sum = [&](int *last) {
+        double sum = 0.0;
 #pragma unroll
-    for (uint32_t j = 0; j < 4; j++)
+        for (uint32_t i = 0; i < 16; i++) sum += part[i];
+        *last = -1;
 #pragma unroll
-        for (uint32_t e = 0; e < 4; e++) {
-            const int x = (int)(chunk * kVerifyChunk + 1024 * j + 4 * tid + e);
-            if (r[j][e] > 0.0) last_r = x;
-            if (w[j][e] > 0.0) last_w = x;
-        }
-    last_r = wave_max(last_r);
-    last_w = wave_max(last_w);
-    if (lane == 0) lasts[0][wave] = last_r, lasts[1][wave] = last_w;
-    __syncthreads();
+        for (uint32_t i = 0; i < 4; i++) *last = lasts[i] > *last ? lasts[i] : *last;
+        return sum;
+    };
+    auto put = [&](uint32_t c, double sum, int last) {   // (one lane)
+        uint64_t *o = reinterpret_cast<uint64_t *>(a.sums + (size_t)s * a.chunks + c);
+        __hip_atomic_store(o, __builtin_bit_cast(uint64_t, sum), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __hip_atomic_store(o + 1, (uint64_t)(int64_t)last, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    };
 
-    // the first wave: this chunk's sums out, the ticket; with the last one the
-    // chunk that the pick falls into, 64 chunks at a time
+    weigh(chunk);
     if (wave == 0) {
-        VerifySum v = {0.0, 0.0, -1, -1};
-#pragma unroll
-        for (uint32_t i = 0; i < 16; i++) {
-            v.rest += part[0][i];
-            v.whole += part[1][i];
-        }
-#pragma unroll
-        for (uint32_t i = 0; i < 4; i++) {
-            v.last_rest = lasts[0][i] > v.last_rest ? lasts[0][i] : v.last_rest;
-            v.last_whole = lasts[1][i] > v.last_whole ? lasts[1][i] : v.last_whole;
-        }
         uint32_t mine = 1;
+        int last;
+        const double sum = chunk_sum(&last);
         if (a.chunks > 1) {
             if (lane == 0) {
                 // complete at device scope before the ticket is taken (no cache-wide fence)
-                uint64_t *o = reinterpret_cast<uint64_t *>(a.sums + blockIdx.x);
-                const uint64_t words[3] = {__builtin_bit_cast(uint64_t, v.rest), __builtin_bit_cast(uint64_t, v.whole),
-                                           (uint64_t)(uint32_t)v.last_whole << 32 | (uint32_t)v.last_rest};
-#pragma unroll
-                for (int i = 0; i < 3; i++) __hip_atomic_store(o + i, words[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                put(chunk, sum, last);
                 __atomic_signal_fence(__ATOMIC_SEQ_CST);
                 __builtin_amdgcn_s_waitcnt(0);
                 __atomic_signal_fence(__ATOMIC_SEQ_CST);
@@ -190,41 +187,44 @@ __global__ __launch_bounds__(256) void verify_kernel(VerifyArgs a) {
             mine = __builtin_amdgcn_readfirstlane(mine);
         }
         if (lane == 0) is_last = mine;
-        if (mine) {
+    }
+    __syncthreads();
+    if (!is_last) return;
+
+    for (;;) {
+        // the chunk that the pick falls into, 64 chunks at a time
+        if (wave == 0) {
             __atomic_signal_fence(__ATOMIC_SEQ_CST);
-            double c_rest, c_whole;   // sums of lane's chunk (this one's own without others), their last places
-            int c_lr, c_lw;
+            double c_sum;   // lane's chunk (without others this one)
+            int c_last;
             auto load_sums = [&](uint32_t c) {
-                c_rest = c_whole = 0.0;
-                c_lr = c_lw = -1;
-                if (a.chunks == 1) {
-                    if (c == 0) c_rest = v.rest, c_whole = v.whole, c_lr = v.last_rest, c_lw = v.last_whole;
-                } else if (c < a.chunks) {
-                    const uint64_t *o = reinterpret_cast<const uint64_t *>(a.sums + (size_t)s * a.chunks + c);
-                    c_rest = __builtin_bit_cast(double, __hip_atomic_load(o, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-                    c_whole = __builtin_bit_cast(double, __hip_atomic_load(o + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-                    const uint64_t l = __hip_atomic_load(o + 2, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                    c_lr = (int)(uint32_t)l;
-                    c_lw = (int)(uint32_t)(l >> 32);
+                int last;
+                const double sum = chunk_sum(&last);
+                c_sum = c == 0 ? sum : 0.0;
+                c_last = c == 0 ? last : -1;
+                if (a.chunks > 1) {
+                    c_sum = 0.0, c_last = -1;
+                    if (c < a.chunks) {
+                        const uint64_t *o = reinterpret_cast<const uint64_t *>(a.sums + (size_t)s * a.chunks + c);
+                        c_sum = __builtin_bit_cast(double, __hip_atomic_load(o, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+                        c_last = (int)__hip_atomic_load(o + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    }
                 }
             };
-            double all_rest = 0.0, all_whole = 0.0;
-            int all_lr = -1, all_lw = -1;
+            double all = 0.0;
+            int last = -1;
             for (uint32_t c0 = 0; c0 < a.chunks; c0 += 64) {
                 load_sums(c0 + lane);
-                all_rest += wave_sum(c_rest);
-                all_whole += wave_sum(c_whole);
-                const int lr = wave_max(c_lr), lw = wave_max(c_lw);
-                all_lr = lr > all_lr ? lr : all_lr;
-                all_lw = lw > all_lw ? lw : all_lw;
+                all += last_lane(wave_scan(c_sum));
+                const int l = wave_max(c_last);
+                last = l > last ? l : last;
             }
-            const bool rest = all_rest > 0.0;   // (rounding may leave p = q at a draft that is not kept: then p itself)
-            const double t = (double)a.u[(size_t)seq * (a.n_draft + 1) + a.n_draft] * (rest ? all_rest : all_whole);
+            const double t = (double)a.u[(size_t)seq * (a.n_draft + 1) + a.n_draft] * all;
             double sum = 0.0;
             uint32_t hit = a.chunks;
             for (uint32_t c0 = 0; c0 < a.chunks; c0 += 64) {
                 if (a.chunks > 64) load_sums(c0 + lane);
-                const double upto = wave_scan(rest ? c_rest : c_whole, lane);
+                const double upto = wave_scan(c_sum);
                 const uint64_t past = __ballot(c0 + lane < a.chunks && sum + upto > t);
                 if (past) {
                     const int l = __builtin_ctzll(past);
@@ -233,33 +233,48 @@ __global__ __launch_bounds__(256) void verify_kernel(VerifyArgs a) {
                     if (l) sum += up;
                     break;
                 }
-                sum += __shfl(upto, 63, 64);
+                sum += last_lane(upto);
             }
             if (lane == 0) {
                 // not passed at all (u, or a rounding, at the very end): the last token that has a weight, if one has
-                const int l = rest ? all_lr : all_lw;
-                token = l < 0 ? YULE_NO_TOKEN : (uint32_t)l;
-                target = t, before = sum, at = hit, of_rest = rest;
+                token = last < 0 ? YULE_NO_TOKEN : (uint32_t)last;
+                target = t, before = sum, at = hit;
+                again = last < 0 && q;
             }
         }
-    }
-    __syncthreads();
-    if (!is_last) return;
-    if (at < a.chunks) {
-        if (a.chunks > 1) weigh(at * kVerifyChunk);   // (one chunk: still there)
         __syncthreads();
-        // the 256 values, then the four, then the value
-        const double *sums = part[of_rest ? 0 : 1];
-        // (sums taken in other orders may round to either side of the target: then the last with a weight)
-        double run_sum = before, sum = before;
+        if (!again) break;
+        // p = q at a draft that is not kept (roundings can leave that, or a draft that is no token): p itself
+        q = nullptr;
+        for (uint32_t c = 0; c < a.chunks; c++) {
+            weigh(c);
+            if (tid == 0 && a.chunks > 1) {
+                int last;
+                const double sum = chunk_sum(&last);
+                put(c, sum, last);
+            }
+            if (c + 1 < a.chunks) __syncthreads();
+        }
+        if (tid == 0) {   // (read by the first wave only, which waits for them here)
+            __atomic_signal_fence(__ATOMIC_SEQ_CST);
+            __builtin_amdgcn_s_waitcnt(0);
+            __atomic_signal_fence(__ATOMIC_SEQ_CST);
+        }
+        __syncthreads();
+    }
+    if (at < a.chunks) {
+        if (a.chunks > 1) weigh(at);   // (one chunk: still there)
+        // The 256 values, then the four, then the value.  (Sums taken in other orders may round to either side of the
+        // target: then the last with a weight.)
+        double run = before, sum = before;
         uint32_t i = 0;
         for (uint32_t k = 0; k < 16; k++) {
-            if (sums[k] > 0.0) {
+            if (part[k] > 0.0) {
                 i = k;
-                sum = run_sum;
-                if (run_sum + sums[k] > target) break;
+                sum = run;
+                if (run + part[k] > target) break;
             }
-            run_sum += sums[k];
+            run += part[k];
         }
         if (wave == (i & 3u)) {
             double mine[4];
@@ -267,22 +282,22 @@ __global__ __launch_bounds__(256) void verify_kernel(VerifyArgs a) {
             for (uint32_t j = 0; j < 4; j++)
                 if (j == i >> 2) {
 #pragma unroll
-                    for (uint32_t e = 0; e < 4; e++) mine[e] = of_rest ? r[j][e] : w[j][e];
+                    for (uint32_t e = 0; e < 4; e++) mine[e] = w[j][e];
                 }
             const double four = (mine[0] + mine[1]) + (mine[2] + mine[3]);
-            const double upto = sum + wave_scan(four, lane);
+            const double upto = sum + wave_scan(four);
             const uint64_t past = __ballot(upto > target && four > 0.0), some = __ballot(four > 0.0);
             const uint32_t l = past ? (uint32_t)__builtin_ctzll(past) : some ? 63u - (uint32_t)__builtin_clzll(some) : 0u;
-            double run = __shfl_up(upto, 1, 64);
-            if (lane == 0) run = sum;
+            double here = __shfl_up(upto, 1, 64);
+            if (lane == 0) here = sum;
             if (lane == l && some) {
-                uint32_t e = 0, pick = 0;
+                uint32_t pick = 0;
                 bool found = false;
 #pragma unroll
-                for (; e < 4; e++) {
-                    run += mine[e];
+                for (uint32_t e = 0; e < 4; e++) {
+                    here += mine[e];
                     if (mine[e] > 0.0 && !found) pick = e;
-                    found = found || run > target;
+                    found = found || here > target;
                 }
                 token = at * kVerifyChunk + 1024 * (i >> 2) + 4 * tid + pick;
             }
