@@ -146,6 +146,13 @@ struct WaveAttn {
         l = 0.f;
     }
 
+    // The queries are there: the compiler, which knows nothing of the copies into
+    // LDS, would otherwise wait for its loads of them inside the loop, with
+    // every copy that is in flight then.
+    __device__ __forceinline__ void wait_queries() {
+#pragma unroll
+        for (uint32_t s = 0; s < NS; s++) asm volatile("" : "+v"(q[s]));
+    }
     // S^T = K Q^T with K's subtile at k
     __device__ __forceinline__ f16v scores(const uint8_t *k, uint32_t lane) const {
         const uint32_t r = lane & 31u, h = lane >> 5;
@@ -282,26 +289,30 @@ struct WaveAttn {
             for (uint32_t i = 0; i < 2 * NL; i++) *reinterpret_cast<i4v *>(lds + 1024 * i + 16 * lane) = i4v{0, 0, 0, 0};
             wait_lds();
         }
+        using No = std::false_type;
+        using Yes = std::true_type;
         // Lane's part of copy i: LDS chunk 64 i + lane of the subtile.  Rows past
         // the last key repeat it (hidden, and the number of copies stays).
         auto copy = [&](const Rows &R, auto is_v, uint32_t at) {
             constexpr uint32_t STEP = decltype(is_v)::value ? 2 : 1;
             const uint8_t *base = uniform(reinterpret_cast<uint64_t>(R.p) + (uint64_t)at * R.stride);
-            const uint32_t last = k1 - at - 1u, ln = opaque(lane) & 63u;
+            const uint32_t last = k1 - at - 1u, ln = opaque(lane) & 63u, dst = lds0 + (decltype(is_v)::value ? SUB : 0u);
+            auto each = [&](auto whole) {
 #pragma unroll
-            for (uint32_t i = 0; i < NL; i++) {
-                const uint32_t L = 64 * i + ln, r = L / C, ch = (L % C) ^ swizzle<C, STEP>(r);
-                if (16 * ch < hb)
-                    copy_to_lds(base, (r < last ? r : last) * R.stride + 16 * ch,
-                                lds0 + (decltype(is_v)::value ? SUB : 0u) + 1024 * i);
-            }
+                for (uint32_t i = 0; i < NL; i++) {
+                    const uint32_t L = 64 * i + ln, r = L / C, ch = (L % C) ^ swizzle<C, STEP>(r);
+                    if (decltype(whole)::value || 16 * ch < hb)
+                        copy_to_lds(base, (r < last ? r : last) * R.stride + 16 * ch, dst + 1024 * i);
+                }
+            };
+            if (hb == RB) each(Yes{});
+            else each(No{});
         };
-        using No = std::false_type;
-        using Yes = std::true_type;
         if (key < k1) {
             copy(K, No{}, key);
             copy(V, Yes{}, key);
         }
+        wait_queries();
         for (; key < k1; key += step) {
             const bool more = key + step < k1;
             wait_copies<NL>();   // K is there
@@ -448,6 +459,7 @@ struct TileAttn {
             }
         };
         copy(k0, 0);
+        w.wait_queries();
         uint32_t buf = 0;
         for (uint32_t key = k0; key < k1; key += KEYS, buf ^= 1u) {
             wait_copies<0>();
