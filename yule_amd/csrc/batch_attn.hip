@@ -78,6 +78,42 @@ __device__ __forceinline__ bool not_finite(i4v x) {
     return bad;
 }
 
+// A key that a slot does not see has weight 0, but 0 times an infinity or a NaN
+// is not 0: where some slots do not see some keys, V's values that are not finite
+// become 0 in LDS (N words of 16 bytes a lane, as the lanes copied them) and are
+// added at the end to those that see them.  Their weights do not matter then.
+// True (in every lane): there were some.
+template <typename T, uint32_t N>
+__device__ __forceinline__ bool drop_not_finite(uint8_t *v, uint32_t lane) {
+    bool bad = false;
+#pragma unroll
+    for (uint32_t i = 0; i < N; i++) bad |= not_finite<T>(*reinterpret_cast<const i4v *>(v + 1024 * i + 16 * lane));
+    if (!__ballot(bad)) return false;
+#pragma unroll 1
+    for (uint32_t i = 0; i < N; i++) {
+        T *x = reinterpret_cast<T *>(v + 1024 * i + 16 * lane);
+#pragma unroll
+        for (uint32_t j = 0; j < 16 / sizeof(T); j++) {
+            const float f = (float)x[j];
+            if (!(__builtin_fabsf(f) < INFINITY)) x[j] = (T)0.f;
+        }
+    }
+    return true;
+}
+// sums of four dims + the values that are not finite of keys k0 .. k1 - 1 (v: key 0's four)
+template <typename T>
+__device__ __forceinline__ f4v add_not_finite(f4v o, const uint8_t *v, uint32_t stride, uint32_t k0, uint32_t k1) {
+    for (uint32_t k = k0; k < k1; k++) {
+        const T *x = reinterpret_cast<const T *>(v + (size_t)k * stride);
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float f = (float)x[j];
+            if (!(__builtin_fabsf(f) < INFINITY)) o[j] += f;
+        }
+    }
+    return o;
+}
+
 // ---- a subtile in LDS: 32 rows of D elements as C 16-byte chunks, chunk c of
 // row r at chunk c ^ swizzle(r) of its row.  P rows fill the 256 bytes of all
 // banks, and the XOR walks the G chunks that a power of two divides off C: 16
@@ -238,48 +274,13 @@ struct WaveAttn {
         }
     }
 
-    // The same, key by key, for a subtile some of whose keys are hidden from some
-    // slots and whose V holds an infinity or a NaN: 0 times that is not 0, so
-    // hidden keys have to be left out, not weighted with 0.  (key0: the
-    // subtile's first key; the slot sees keys below lim.)
-    __device__ __forceinline__ void values_seen(const f16v &s, const uint8_t *v, uint32_t tid, uint32_t key0,
-                                                uint32_t lim) {
-        const uint32_t lane = opaque(tid) & 63u, h = lane >> 5;
-#pragma unroll 1
-        for (uint32_t k = 0; k < 32; k++) {
-            const uint32_t at = 4 * (k >> 3) + (k & 3u);
-            float p = 0.f;
-#pragma unroll
-            for (int i = 0; i < 16; i++) p = at == (uint32_t)i ? s[i] : p;
-            p = __shfl(p, 32 * ((k >> 2) & 1u) + (lane & 31u), 64);
-            if (key0 + k >= lim) continue;
-#pragma unroll
-            for (uint32_t t = 0; t < DT; t++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    if (i % 4 == 0) __builtin_amdgcn_sched_barrier(0);   // (few values in registers at a time)
-                    const uint32_t d = 32 * t + 8 * (i / 4) + 4 * h + i % 4;
-                    const uint8_t *x = v + k * RB + (((d * SZ / 16) ^ swizzle<C, 2>(k)) << 4) + d * SZ % 16;
-                    o[t][i] = fmaf(p, (float)*reinterpret_cast<const T *>(x), o[t][i]);
-                }
-        }
-    }
-
-    // some element of V's subtile is infinite or NaN (the same in every lane)
-    __device__ __forceinline__ static bool holds_not_finite(const uint8_t *v, uint32_t lane) {
-        bool bad = false;
-#pragma unroll
-        for (uint32_t i = 0; i < NL; i++) bad |= not_finite<T>(*reinterpret_cast<const i4v *>(v + 1024 * i + 16 * lane));
-        return __ballot(bad) != 0;
-    }
-
     // Keys key, key + step, .. < k1 in subtiles of 32 (lds: this wave's K subtile
-    // and V subtile).  A slot sees keys below lim; every slot sees those below
-    // lim_all.  The next K subtile is on its way while this one's softmax and
+    // and V subtile).  A slot sees keys below lim, every slot those below lim_all
+    // <= k1.  The next K subtile is on its way while this one's softmax and
     // product with V run, the next V subtile during the next scores: copies
     // complete in order, so "at most NL in flight" says that the older of the
-    // two has landed.
-    __device__ __forceinline__ void walk(const Rows &K, const Rows &V, uint32_t hb, uint32_t key, uint32_t step,
+    // two has landed.  True: drop_not_finite dropped something.
+    __device__ __forceinline__ bool walk(const Rows &K, const Rows &V, uint32_t hb, uint32_t key, uint32_t step,
                                          uint32_t k1, uint32_t lim, uint32_t lim_all, uint8_t *lds, uint32_t lane,
                                          float c) {
         const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)reinterpret_cast<uintptr_t>((lds_b)lds));
@@ -313,22 +314,25 @@ struct WaveAttn {
             copy(V, Yes{}, key);
         }
         wait_queries();
-        for (; key < k1; key += step) {
+        bool dropped = false;
+        auto subtile = [&](auto masked) {
             const bool more = key + step < k1;
             wait_copies<NL>();   // K is there
             f16v s[1] = {scores(lds, opaque(lane) & 63u)};
             wait_lds();
             if (more) copy(K, No{}, key + step);
-            const bool masked = key + 32 > lim_all;
-            if (masked) hide(s[0], key, lim, lane);
+            if (decltype(masked)::value) hide(s[0], key, lim, lane);
             softmax(s, c);
             if (more) wait_copies<NL>();   // V is there
             else wait_copies<0>();
-            if (masked && holds_not_finite(vt, lane)) values_seen(s[0], vt, lane, key, lim);
-            else values(s[0], vt, opaque(lane) & 63u);
+            if (decltype(masked)::value) dropped |= drop_not_finite<T, NL>(vt, lane);
+            values(s[0], vt, opaque(lane) & 63u);
             wait_lds();
             if (more) copy(V, Yes{}, key + step);
-        }
+        };
+        for (; key + 32 <= lim_all; key += step) subtile(No{});
+        for (; key < k1; key += step) subtile(Yes{});
+        return dropped;
     }
 };
 
@@ -343,6 +347,7 @@ struct BlockAttn {
     struct Shared {
         __align__(1024) uint8_t tiles[NW][2 * W::SUB];
         float m[NW][32], l[NW][32];
+        uint32_t lim[32], dropped[NW];
     };
 
     // out(slot of 32, dim, four sums, maximum, weight): joined over the waves
@@ -354,12 +359,15 @@ struct BlockAttn {
         const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         W w;
         w.init(qrow, hb, h);
-        w.walk(K, V, hb, k0 + 32 * wave, 32 * NW, k1, lim, lim_all, sh.tiles[wave], lane, c);
+        lim_all = lim_all < k1 ? lim_all : k1;
+        const bool dropped = w.walk(K, V, hb, k0 + 32 * wave, 32 * NW, k1, lim, lim_all, sh.tiles[wave], lane, c);
         const float l = w.l + __shfl_xor(w.l, 32, 64);
         if (h == 0) {
             sh.m[wave][r32] = w.m;
             sh.l[wave][r32] = l;
+            sh.lim[r32] = lim;   // (the same from every wave)
         }
+        if (lane == 0) sh.dropped[wave] = dropped;
         // the wave's subtiles make room for its sums, f32 [32][D], chunks XORed with the row (the writes of
         // eight lanes lie in different banks)
         uint8_t *const ob = sh.tiles[wave];
@@ -370,6 +378,9 @@ struct BlockAttn {
                 *reinterpret_cast<f4v *>(ob + r32 * D * 4 + (((8 * t + 2 * a + h) ^ (r32 & 7u)) << 4)) =
                     f4v{w.o[t][4 * a], w.o[t][4 * a + 1], w.o[t][4 * a + 2], w.o[t][4 * a + 3]};
         __syncthreads();
+        uint32_t any = 0;
+#pragma unroll
+        for (uint32_t x = 0; x < NW; x++) any |= sh.dropped[x];
         for (uint32_t i = tid; i < 32 * (D / 4); i += 64 * NW) {
             const uint32_t r = i / (D / 4), ch = i % (D / 4);
             float M = sh.m[0][r];
@@ -385,6 +396,9 @@ struct BlockAttn {
                 L += f * sh.l[x][r];
                 acc += f * o;
             }
+            // (dropped from the first subtile on that some slot does not see whole)
+            if (any && 16 * ch < 4 * hb / W::SZ)
+                acc = add_not_finite<T>(acc, V.p + 4 * ch * W::SZ, V.stride, lim_all < k0 ? k0 : lim_all - (lim_all - k0) % 32, sh.lim[r]);
             out(r, 4 * ch, acc, M, L);
         }
     }
@@ -401,15 +415,17 @@ struct TileAttn {
     static_assert(NSUB * W::NL % NW == 0);
     struct Shared {
         __align__(1024) uint8_t kv[2][2][TILE];
+        uint32_t dropped[NW];
     };
 
-    // Every wave: its slots' keys below k1 (the workgroup's); the wave's slots see
-    // keys below lim (each lane's own), all of them those below lim_lo, none those
-    // from lim_hi (0: the wave has no slots).  out(dim, four sums, maximum, weight) of the lane's slot.
+    // Keys k0 .. k1 - 1 of the workgroup, every slot of which sees those below
+    // lim_all; the wave's slots see keys below lim (each lane's own), all of them
+    // those below lim_lo, none those from lim_hi (0: the wave has no slots).
+    // out(dim, four sums, maximum, weight) of the lane's slot.
     template <typename OUT>
     __device__ __forceinline__ static void run(Shared &sh, const uint8_t *qrow, const Rows &K, const Rows &V, uint32_t hb,
-                                               uint32_t k0, uint32_t k1, uint32_t lim, uint32_t lim_lo, uint32_t lim_hi,
-                                               float c, OUT out) {
+                                               uint32_t k0, uint32_t k1, uint32_t lim, uint32_t lim_all, uint32_t lim_lo,
+                                               uint32_t lim_hi, float c, OUT out) {
         constexpr uint32_t RB = W::RB, C = W::C, SUB = W::SUB;
         const uint32_t tid = threadIdx.x, lane = tid & 63u, h = lane >> 5;
         const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -460,40 +476,54 @@ struct TileAttn {
         };
         copy(k0, 0);
         w.wait_queries();
-        uint32_t buf = 0;
-        for (uint32_t key = k0; key < k1; key += KEYS, buf ^= 1u) {
+        uint32_t buf = 0, key = k0;
+        bool dropped = false;
+        auto next = [&]() {   // the tile at key is there, the next one on its way
             wait_copies<0>();
+            if (key + KEYS > lim_all)   // (each wave looks at what it copied)
+                dropped |= drop_not_finite<T, NC>(&sh.kv[buf][1][0] + 1024 * NC * wave, lane);
             wait_lds();
             __builtin_amdgcn_s_barrier();   // every wave's copies are there, and nobody reads the other half
             __atomic_signal_fence(__ATOMIC_SEQ_CST);
             if (key + KEYS < k1) copy(key + KEYS, buf ^ 1u);
+        };
+        for (; key + KEYS <= lim_lo; key += KEYS, buf ^= 1u) {   // tiles that every slot of the wave sees whole
+            next();
             const uint8_t *kt = &sh.kv[buf][0][0], *vt = &sh.kv[buf][1][0];
-            if (key + KEYS <= lim_lo) {
-                f16v s[NSUB];
+            f16v s[NSUB];
 #pragma unroll
-                for (uint32_t n = 0; n < NSUB; n++) s[n] = w.scores(kt + n * SUB, lane);
-                w.softmax(s, c);
+            for (uint32_t n = 0; n < NSUB; n++) s[n] = w.scores(kt + n * SUB, lane);
+            w.softmax(s, c);
 #pragma unroll
-                for (uint32_t n = 0; n < NSUB; n++) w.values(s[n], vt + n * SUB, lane);
-            } else {
+            for (uint32_t n = 0; n < NSUB; n++) w.values(s[n], vt + n * SUB, lane);
+        }
+        for (; key < k1; key += KEYS, buf ^= 1u) {   // and the others, subtile by subtile
+            next();
 #pragma unroll 1
-                for (uint32_t n = 0; n < NSUB; n++) {
-                    const uint32_t key0 = key + 32 * n;
-                    if (key0 >= lim_hi) break;
-                    f16v s[1] = {w.scores(kt + n * SUB, lane)};
-                    W::hide(s[0], key0, lim, lane);
-                    w.softmax(s, c);
-                    if (W::holds_not_finite(vt + n * SUB, lane)) w.values_seen(s[0], vt + n * SUB, lane, key0, lim);
-                    else w.values(s[0], vt + n * SUB, opaque(lane) & 63u);
-                }
+            for (uint32_t n = 0; n < NSUB; n++) {
+                if (key + 32 * n >= lim_hi) break;
+                const uint32_t ln = opaque(lane) & 63u;
+                f16v s[1] = {w.scores(&sh.kv[buf][0][n * SUB], ln)};
+                W::hide(s[0], key + 32 * n, lim, lane);
+                w.softmax(s, c);
+                w.values(s[0], &sh.kv[buf][1][n * SUB], ln);
             }
         }
         const float l = w.l + __shfl_xor(w.l, 32, 64);
+        if (lane == 0) sh.dropped[wave] = dropped;
+        __syncthreads();
+        const uint32_t any = sh.dropped[0] | sh.dropped[1] | sh.dropped[2] | sh.dropped[3];
 #pragma unroll
         for (uint32_t t = 0; t < W::DT; t++)
 #pragma unroll
-            for (uint32_t a = 0; a < 4; a++)
-                out(32 * t + 8 * a + 4 * h, f4v{w.o[t][4 * a], w.o[t][4 * a + 1], w.o[t][4 * a + 2], w.o[t][4 * a + 3]}, w.m, l);
+            for (uint32_t a = 0; a < 4; a++) {
+                const uint32_t d = 32 * t + 8 * a + 4 * h;
+                f4v o = {w.o[t][4 * a], w.o[t][4 * a + 1], w.o[t][4 * a + 2], w.o[t][4 * a + 3]};
+                // (dropped from the first tile on that some slot of the workgroup does not see whole)
+                if (any && d * W::SZ < hb)
+                    o = add_not_finite<T>(o, V.p + d * W::SZ, V.stride, lim_all < k0 ? k0 : lim_all - (lim_all - k0) % KEYS, lim);
+                out(d, o, w.m, l);
+            }
     }
 };
 
@@ -600,7 +630,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 
     const Rows K = {a.k + (size_t)row0 * a.ks + (size_t)kvh * hb, a.ks}, V = {a.v + (size_t)row0 * a.vs + (size_t)kvh * hb, a.vs};
     const bool any = first_w <= last, own = first_w + (lane & 31u) <= last;
     uint8_t *const out = a.out + (size_t)(row0 + r) * a.os + head;
-    B::run(sh, a.q + (size_t)(row0 + r) * a.qs + head, K, V, hb, 0, last / g + 1u, r + 1u, any ? first_w / g + 1u : 0u,
+    B::run(sh, a.q + (size_t)(row0 + r) * a.qs + head, K, V, hb, 0, last / g + 1u, r + 1u, slot0 / g + 1u, any ? first_w / g + 1u : 0u,
            any ? last_w / g + 1u : 0u, a.s.c, [&](uint32_t d, f4v o, float, float L) {
                if (own && d < a.s.hd) store4<T>(out, d, o * (L == 0.f ? 0.f : 1.0f / L));
            });
@@ -648,7 +678,7 @@ __global__ __launch_bounds__((64 * BlockAttn<T, D>::NW))
             const uint32_t first = 128 * tile + 32 * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), slot = first + (lane & 31u);
             const uint32_t mine = slot < slots ? slot : slots - 1u;
             const size_t at = part + pair(mine);
-            P::run(sh.tile, query(mine), K, V, hb, k0, k1, k1, first < slots ? k1 : 0u, first < slots ? k1 : 0u, a.s.c,
+            P::run(sh.tile, query(mine), K, V, hb, k0, k1, k1, k1, first < slots ? k1 : 0u, first < slots ? k1 : 0u, a.s.c,
                    [&](uint32_t d, f4v o, float M, float L) {
                        if (slot >= slots || d >= a.s.hd) return;
                        if (d == 0) a.ml[at] = make_float2(M, L);
