@@ -120,6 +120,10 @@ PROMPTS = [
     (2, 2, 256, [40, 3], 1),
     (3, 1, 8, [129, 2], 0),
     (4, 1, 96, [130], 0),
+    (2, 1, 32, [70, 9], 0),
+    (2, 1, 136, [50, 4], 2),
+    (1, 1, 168, [35], 0),
+    (2, 2, 200, [33, 1], 0),
     (32, 4, 64, [17, 100], 0),
 ]
 
@@ -243,6 +247,8 @@ PREFIXES = [
     (4, 1, 64, 77, 0, [0, 9], 2),                  # no tail at all
     (2, 2, 8, 520, 600, [600, 513, 99, 2 ** 32 - 1], 1),   # more than one chunk of each; a length above the capacity
     (2, 1, 64, 10, 80, [80, 70], 64),
+    (2, 2, 152, 90, 20, [20, 7], 2),
+    (4, 1, 24, 70, 33, [33, 0, 5], 1),
 ]
 
 

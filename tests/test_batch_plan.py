@@ -41,7 +41,11 @@ int main() {
     CHECK(check_heads(4, 4, 0) && check_heads(4, 4, 12) && check_heads(4, 4, 264) && check_heads(8192, 8, 64));
     CHECK(attn_elem_bytes(YULE_DTYPE_F32) == 4 && attn_elem_bytes(YULE_DTYPE_F16) == 2 &&
           attn_elem_bytes(YULE_DTYPE_BF16) == 2 && attn_elem_bytes(YULE_DTYPE_Q8_0) == 0);
-    for (uint32_t hd = 8; hd <= 256; hd += 8) CHECK(attn_padded_dim(hd) >= hd && attn_padded_dim(hd) % 32 == 0);
+    for (uint32_t hd = 8; hd <= 256; hd += 8) {
+        const uint32_t d4 = attn_padded_dim(hd, 4), d2 = attn_padded_dim(hd, 2);
+        CHECK(d4 >= hd && d4 % 32 == 0 && d4 - hd < 32);   // f32: some of the head in every piece of 32 dims
+        CHECK(d2 >= hd && (d2 == 64 || d2 == 96 || d2 == 128 || d2 == 256));
+    }
     // plans: chunks cover the keys once, jobs fit, results lie in the workspace
     unsigned seed = 1;
     auto rnd = [&](uint32_t n) { seed = seed * 1664525u + 1013904223u; return (seed >> 8) % n; };

@@ -158,11 +158,44 @@ struct Rows {
     uint32_t stride;
 };
 
+// The scores of N subtiles into probabilities against the new running maximum m of
+// c S (the product and the difference round once, in the fused multiply-add); the
+// weight's sum l (this lane's keys) and the sums o rescaled where it moved.
+template <uint32_t N, uint32_t DT>
+__device__ __forceinline__ void online_softmax(f16v (&s)[N], f16v (&o)[DT], float &m, float &l, float c) {
+    float cm = s[0][0];
+#pragma unroll
+    for (uint32_t n = 0; n < N; n++)
+#pragma unroll
+        for (int i = n ? 0 : 1; i < 16; i++) cm = fmaxf(cm, s[n][i]);
+    cm = fmaxf(cm, __shfl_xor(cm, 32, 64)) * c;
+    if (__ballot(cm > m)) {
+        const float mn = fmaxf(m, cm);
+        // (m = -inf: nothing was added yet, and the factor multiplies zeros)
+        const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= alpha;
+#pragma unroll
+        for (uint32_t t = 0; t < DT; t++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[t][i] *= alpha;
+    }
+    const float mb = m == -INFINITY ? 0.f : m;   // nothing seen yet: weights of 0
+#pragma unroll
+    for (uint32_t n = 0; n < N; n++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            s[n][i] = __builtin_amdgcn_exp2f(fmaf(s[n][i], c, -mb));
+            l += s[n][i];
+        }
+}
+
 // ---- one wave: 32 slots over keys key0, key0 + step, .. < k1 (subtiles of 32)
 template <typename T, uint32_t D>
 struct WaveAttn {
     static constexpr uint32_t SZ = sizeof(T), RB = D * SZ, C = RB / 16, SUB = 32 * RB;
     static constexpr uint32_t NL = SUB / 1024, NS = RB / 32, DT = D / 32;
+    static constexpr uint32_t LDS = 2 * SUB;   // bytes of a wave that walks by itself
     i4v q[NS];    // bytes 32 s + 16 h .. of this lane's slot's query
     f16v o[DT];   // O^T, unnormalised: dim 32 t + 8 (i / 4) + 4 h + i % 4
     float m, l;   // running maximum of c S; this lane's share of the weight's sum
@@ -207,52 +240,10 @@ struct WaveAttn {
             if (key0 + 8 * (i / 4) + 4 * (lane >> 5) + i % 4 >= lim) s[i] = -INFINITY;
     }
 
-    // the subtiles' scores into probabilities, sums rescaled where a maximum moved
-    template <uint32_t N>
-    __device__ __forceinline__ void softmax(f16v (&s)[N], float c) {
-        float cm = s[0][0];
-#pragma unroll
-        for (uint32_t n = 0; n < N; n++)
-#pragma unroll
-            for (int i = n ? 0 : 1; i < 16; i++) cm = fmaxf(cm, s[n][i]);
-        cm = fmaxf(cm, __shfl_xor(cm, 32, 64)) * c;
-        if (__ballot(cm > m)) {
-            const float mn = fmaxf(m, cm);
-            // (m = -inf: nothing was added yet, and the factor multiplies zeros)
-            const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
-            m = mn;
-            l *= alpha;
-#pragma unroll
-            for (uint32_t t = 0; t < DT; t++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) o[t][i] *= alpha;
-        }
-        const float mb = m == -INFINITY ? 0.f : m;   // nothing seen yet: weights of 0
-#pragma unroll
-        for (uint32_t n = 0; n < N; n++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-                s[n][i] = __builtin_amdgcn_exp2f(fmaf(s[n][i], c, -mb));
-                l += s[n][i];
-            }
-    }
-
     // O^T += V^T P^T with V's subtile at v
     __device__ __forceinline__ void values(const f16v &s, const uint8_t *v, uint32_t lane) {
         const uint32_t h = lane >> 5;
-        if constexpr (SZ == 4) {
-            const uint32_t d = lane & 31u;
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-                const uint32_t r = 8 * (i / 4) + 4 * h + i % 4;
-#pragma unroll
-                for (uint32_t t = 0; t < DT; t++) {
-                    const float a = *reinterpret_cast<const float *>(
-                        v + r * RB + (((8 * t + (d >> 2)) ^ swizzle<C, 2>(r)) << 4) + 4 * (d & 3u));
-                    o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, s[i], o[t], 0, 0, 0);
-                }
-            }
-        } else {
+        {
             // the transposing read gives lane l of 16 column l of the four rows that lanes 4 r .. 4 r + 3 point
             // to: here the dims of V^T's rows from four keys
             const uint32_t e = lane & 15u, g = lane >> 4;
@@ -322,7 +313,7 @@ struct WaveAttn {
             wait_lds();
             if (more) copy(K, No{}, key + step);
             if (decltype(masked)::value) hide(s[0], key, lim, lane);
-            softmax(s, c);
+            online_softmax<1, DT>(s, o, m, l, c);
             if (more) wait_copies<NL>();   // V is there
             else wait_copies<0>();
             if (decltype(masked)::value) dropped |= drop_not_finite<T, NL>(vt, lane);
@@ -336,16 +327,119 @@ struct WaveAttn {
     }
 };
 
+// ---- the same wave for f32, whose products take four times as long per byte and
+// whose rows take twice the LDS: K and V pass through a ring of D / 32 pieces, 32
+// keys x 32 dims each, that holds one subtile of either.  Piece j is replaced by
+// the piece D / 32 further on as soon as it has been used, so copies are always on
+// their way, and half the LDS allows twice the waves: one wave's softmax and waits
+// lie under the others' products.
+template <uint32_t D>
+struct WaveAttn<float, D> {
+    static constexpr uint32_t SZ = 4, NS = D / 8, DT = D / 32, C = 8, PIECE = 4096, LDS = DT * PIECE;
+    i4v q[NS];    // as above
+    f16v o[DT];
+    float m, l;
+
+    __device__ __forceinline__ void init(const uint8_t *qrow, uint32_t hb, uint32_t h) {
+#pragma unroll
+        for (uint32_t s = 0; s < NS; s++) {
+            const uint32_t at = 32 * s + 16 * h;
+            q[s] = i4v{0, 0, 0, 0};
+            if (at < hb) q[s] = *reinterpret_cast<const i4v *>(qrow + at);
+        }
+#pragma unroll
+        for (uint32_t t = 0; t < DT; t++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[t][i] = 0.f;
+        m = -INFINITY;
+        l = 0.f;
+    }
+
+    __device__ __forceinline__ bool walk(const Rows &K, const Rows &V, uint32_t hb, uint32_t key, uint32_t step,
+                                         uint32_t k1, uint32_t lim, uint32_t lim_all, uint8_t *lds, uint32_t lane,
+                                         float c) {
+        const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)reinterpret_cast<uintptr_t>((lds_b)lds));
+        if (hb < D * 4) {   // dims past the head stay zero: copies leave them out
+#pragma unroll
+            for (uint32_t i = 0; i < LDS / 1024; i++) *reinterpret_cast<i4v *>(lds + 1024 * i + 16 * lane) = i4v{0, 0, 0, 0};
+            wait_lds();
+        }
+        // Piece j of the subtile at key `at`: dims 32 j .. of K, then of V.  Lane's part of copy i: chunk lane % 8 of
+        // row 8 i + lane / 8.  Rows past the last key repeat it (hidden, and the number of copies stays).
+        auto copy = [&](uint32_t at, uint32_t j) {
+            const bool is_v = j >= DT;
+            const Rows &R = is_v ? V : K;
+            const uint8_t *base = uniform(reinterpret_cast<uint64_t>(R.p) + (uint64_t)at * R.stride + 128 * (j % DT));
+            const uint32_t last = k1 - at - 1u, ln = opaque(lane) & 63u;
+            const uint32_t left = hb - 128 * (j % DT);   // (hd > D - 32: some of every piece)
+            auto each = [&](auto whole) {
+#pragma unroll
+                for (uint32_t i = 0; i < 4; i++) {
+                    const uint32_t r = 8 * i + (ln >> 3), ch = 16 * ((ln & 7u) ^ (is_v ? swizzle<C, 2>(r) : swizzle<C, 1>(r)));
+                    if (decltype(whole)::value || ch < left)
+                        copy_to_lds(base, (r < last ? r : last) * R.stride + ch, lds0 + PIECE * (j % DT) + 1024 * i);
+                }
+            };
+            if (hb == D * 4) each(std::true_type{});
+            else each(std::false_type{});
+        };
+        if (key < k1) {
+#pragma unroll
+            for (uint32_t j = 0; j < DT; j++) copy(key, j);
+        }
+#pragma unroll
+        for (uint32_t s = 0; s < NS; s++) asm volatile("" : "+v"(q[s]));   // (as wait_queries)
+        bool dropped = false;
+        auto subtile = [&](auto masked) {
+            const bool more = key + step < k1;
+            f16v s[1];
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[0][i] = 0.f;
+#pragma unroll
+            for (uint32_t j = 0; j < DT; j++) {   // S^T += K Q^T
+                wait_copies<4 * (DT - 1)>();
+                const uint32_t ln = opaque(lane) & 63u, r = ln & 31u, h = ln >> 5;
+                const uint8_t *k = lds + PIECE * j + 128 * r;
+#pragma unroll
+                for (uint32_t st = 0; st < 4; st++)
+                    s[0] = mma16<float>(*reinterpret_cast<const i4v *>(k + (((2 * st + h) ^ swizzle<C, 1>(r)) << 4)), q[4 * j + st], s[0]);
+                wait_lds();
+                copy(key, DT + j);
+            }
+            if (decltype(masked)::value) WaveAttn<_Float16, D>::hide(s[0], key, lim, lane);
+            online_softmax<1, DT>(s, o, m, l, c);
+#pragma unroll
+            for (uint32_t j = 0; j < DT; j++) {   // O^T += V^T P^T
+                if (more) wait_copies<4 * (DT - 1)>();
+                else wait_copies<0>();
+                uint8_t *v = lds + PIECE * j;
+                if (decltype(masked)::value) dropped |= drop_not_finite<float, 4>(v, lane);
+                const uint32_t ln = opaque(lane) & 63u, d = ln & 31u, h = ln >> 5;
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const uint32_t r = 8 * (i / 4) + 4 * h + i % 4;
+                    const float a = *reinterpret_cast<const float *>(v + 128 * r + (((d >> 2) ^ swizzle<C, 2>(r)) << 4) + 4 * (d & 3u));
+                    o[j] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, s[0][i], o[j], 0, 0, 0);
+                }
+                wait_lds();
+                if (more) copy(key + step, j);
+            }
+        };
+        for (; key + 32 <= lim_all; key += step) subtile(std::false_type{});
+        for (; key < k1; key += step) subtile(std::true_type{});
+        return dropped;
+    }
+};
+
 // ---- a workgroup: NW waves share 32 slots and take the keys' subtiles in turn
 template <typename T, uint32_t D>
 struct BlockAttn {
     using W = WaveAttn<T, D>;
-    // waves whose subtiles fit the LDS (f32 heads of 256 dims: 64 KB a wave)
-    static constexpr uint32_t NW = 2 * W::SUB * 4 <= 131072 ? 4 : 2;
+    static constexpr uint32_t NW = 4;
     // waves a SIMD that the LDS has room for: the registers are to allow them too
-    static constexpr uint32_t WAVES = 2 * W::SUB * 4 <= 65536 ? 2 : 1;
+    static constexpr uint32_t WAVES = W::LDS <= 8192 ? 4 : W::LDS <= 12288 ? 3 : W::LDS <= 16384 ? 2 : 1;
     struct Shared {
-        __align__(1024) uint8_t tiles[NW][2 * W::SUB];
+        __align__(1024) uint8_t tiles[NW][W::LDS];
         float m[NW][32], l[NW][32];
         uint32_t lim[32], dropped[NW];
     };
@@ -493,7 +587,7 @@ struct TileAttn {
             f16v s[NSUB];
 #pragma unroll
             for (uint32_t n = 0; n < NSUB; n++) s[n] = w.scores(kt + n * SUB, lane);
-            w.softmax(s, c);
+            online_softmax<NSUB, W::DT>(s, w.o, w.m, w.l, c);
 #pragma unroll
             for (uint32_t n = 0; n < NSUB; n++) w.values(s[n], vt + n * SUB, lane);
         }
@@ -505,7 +599,7 @@ struct TileAttn {
                 const uint32_t ln = opaque(lane) & 63u;
                 f16v s[1] = {w.scores(&sh.kv[buf][0][n * SUB], ln)};
                 W::hide(s[0], key + 32 * n, lim, lane);
-                w.softmax(s, c);
+                online_softmax<1, W::DT>(s, w.o, w.m, w.l, c);
                 w.values(s[0], &sh.kv[buf][1][n * SUB], ln);
             }
         }
@@ -653,7 +747,7 @@ template <typename T, uint32_t D, bool TILE>
 __global__ __launch_bounds__((64 * BlockAttn<T, D>::NW))
     __attribute__((amdgpu_waves_per_eu(BlockAttn<T, D>::WAVES))) void prefix_attn_kernel(PrefixArgs a) {
     using B = BlockAttn<T, D>;
-    using P = TileAttn<T, D>;
+    using P = TileAttn<typename std::conditional<TILE, T, _Float16>::type, TILE ? D : 64>;
     __shared__ union {
         typename B::Shared block;
         typename std::conditional<TILE, typename P::Shared, char>::type tile;
@@ -790,7 +884,16 @@ __global__ __launch_bounds__(NT) void prefix_join_kernel(const float2 *__restric
 template <typename F>
 static void by_shape(uint32_t dtype, uint32_t hd, F f) {
     auto dims = [&](auto t) {
-        switch (attn_padded_dim(hd)) {
+        const uint32_t d = attn_padded_dim(hd, sizeof(t));
+        if constexpr (sizeof(t) == 4) {
+            switch (d) {
+            case 32: f(t, std::integral_constant<uint32_t, 32>{}); return;
+            case 160: f(t, std::integral_constant<uint32_t, 160>{}); return;
+            case 192: f(t, std::integral_constant<uint32_t, 192>{}); return;
+            case 224: f(t, std::integral_constant<uint32_t, 224>{}); return;
+            }
+        }
+        switch (d) {
         case 64: f(t, std::integral_constant<uint32_t, 64>{}); break;
         case 96: f(t, std::integral_constant<uint32_t, 96>{}); break;
         case 128: f(t, std::integral_constant<uint32_t, 128>{}); break;
@@ -817,7 +920,7 @@ static int launch_prompt(hipStream_t s, const PromptArgs &a, uint32_t dtype, uin
                 return;
             }
         }
-        hipLaunchKernelGGL((prompt_attn_kernel<T, D>), grid, dim3(64 * BlockAttn<T, D>::NW), 0, s, a);
+        hipLaunchKernelGGL((prompt_attn_kernel<T, D>), grid, dim3(256), 0, s, a);
     });
     return check_launch("prompt_attn");
 }
@@ -832,7 +935,7 @@ static int launch_prefix(hipStream_t s, const PrefixArgs &a, uint32_t dtype, uin
                 return;
             }
         }
-        hipLaunchKernelGGL((prefix_attn_kernel<T, D, false>), dim3((uint32_t)workgroups), dim3(64 * BlockAttn<T, D>::NW), 0, s, a);
+        hipLaunchKernelGGL((prefix_attn_kernel<T, D, false>), dim3((uint32_t)workgroups), dim3(256), 0, s, a);
     });
     return check_launch("prefix_attn");
 }

@@ -17,8 +17,12 @@ inline uint32_t attn_elem_bytes(uint32_t dtype) {
     return dtype == YULE_DTYPE_F32 ? 4u : dtype == YULE_DTYPE_F16 || dtype == YULE_DTYPE_BF16 ? 2u : 0u;
 }
 
-// the head size that the kernels are built for (dims past head_dim are zeros in registers and LDS)
-inline uint32_t attn_padded_dim(uint32_t hd) { return hd <= 64 ? 64u : hd <= 96 ? 96u : hd <= 128 ? 128u : 256u; }
+// the head size that the kernels are built for (dims past head_dim are zeros in
+// registers and LDS); f32: the next multiple of 32, so that every piece of 32
+// dims holds some of the head
+inline uint32_t attn_padded_dim(uint32_t hd, uint32_t elem) {
+    return elem == 4 ? (hd + 31) / 32 * 32 : hd <= 64 ? 64u : hd <= 96 ? 96u : hd <= 128 ? 128u : 256u;
+}
 
 // Rows r < n_rows, each `width` elements of `elem` bytes, of a buffer of
 // buf_bytes: nullptr, or what is wrong.  align: bytes that every row starts at
