@@ -364,24 +364,41 @@ struct WaveAttn<float, D> {
             for (uint32_t i = 0; i < LDS / 1024; i++) *reinterpret_cast<i4v *>(lds + 1024 * i + 16 * lane) = i4v{0, 0, 0, 0};
             wait_lds();
         }
-        // Piece j of the subtile at key `at`: dims 32 j .. of K, then of V.  Lane's part of copy i: chunk lane % 8 of
-        // row 8 i + lane / 8.  Rows past the last key repeat it (hidden, and the number of copies stays).
+        // f32 products keep the vector units from anything else (measured: their
+        // times add up), so addresses are worked out once: of this lane's part of
+        // the four copies of a piece (chunk lane % 8 of row 8 i + lane / 8), and of
+        // its operands in a piece (from where the other rows' are constants away).
+        uint32_t off[2][4], ka[4], va[2];
+        {
+            const uint32_t lr = lane >> 3, r = lane & 31u, h = lane >> 5;
+#pragma unroll
+            for (uint32_t i = 0; i < 4; i++) {
+                off[0][i] = (8 * i + lr) * K.stride + 16 * ((lane & 7u) ^ swizzle<C, 1>(8 * i + lr));
+                off[1][i] = (8 * i + lr) * V.stride + 16 * ((lane & 7u) ^ swizzle<C, 2>(8 * i + lr));
+                ka[i] = 128 * r + (((2 * i + h) ^ swizzle<C, 1>(r)) << 4);
+            }
+            // row 8 (i / 4) + 4 h + i % 4: its swizzle is that of 4 h + i % 4
+#pragma unroll
+            for (uint32_t i = 0; i < 2; i++)
+                va[i] = 128 * 4 * h + (((r >> 2) ^ swizzle<C, 2>(4 * h + 2 * i)) << 4) + 4 * (r & 3u);
+        }
+        // Piece j of the subtile at key `at`: dims 32 j .. of K, then of V.
         auto copy = [&](uint32_t at, uint32_t j) {
             const bool is_v = j >= DT;
             const Rows &R = is_v ? V : K;
             const uint8_t *base = uniform(reinterpret_cast<uint64_t>(R.p) + (uint64_t)at * R.stride + 128 * (j % DT));
-            const uint32_t last = k1 - at - 1u, ln = opaque(lane) & 63u;
-            const uint32_t left = hb - 128 * (j % DT);   // (hd > D - 32: some of every piece)
-            auto each = [&](auto whole) {
+            const uint32_t dst = lds0 + PIECE * (j % DT), left = hb - 128 * (j % DT);   // (hd > D - 32: some of every piece)
+            if (k1 - at >= 32 && left >= 128) {
+#pragma unroll
+                for (uint32_t i = 0; i < 4; i++) copy_to_lds(base, off[is_v][i], dst + 1024 * i);
+            } else {   // rows past the last key repeat it (hidden, and the number of copies stays)
+                const uint32_t last = k1 - at - 1u, ln = opaque(lane) & 63u;
 #pragma unroll
                 for (uint32_t i = 0; i < 4; i++) {
                     const uint32_t r = 8 * i + (ln >> 3), ch = 16 * ((ln & 7u) ^ (is_v ? swizzle<C, 2>(r) : swizzle<C, 1>(r)));
-                    if (decltype(whole)::value || ch < left)
-                        copy_to_lds(base, (r < last ? r : last) * R.stride + ch, lds0 + PIECE * (j % DT) + 1024 * i);
+                    if (ch < left) copy_to_lds(base, (r < last ? r : last) * R.stride + ch, dst + 1024 * i);
                 }
-            };
-            if (hb == D * 4) each(std::true_type{});
-            else each(std::false_type{});
+            }
         };
         if (key < k1) {
 #pragma unroll
@@ -398,11 +415,9 @@ struct WaveAttn<float, D> {
 #pragma unroll
             for (uint32_t j = 0; j < DT; j++) {   // S^T += K Q^T
                 wait_copies<4 * (DT - 1)>();
-                const uint32_t ln = opaque(lane) & 63u, r = ln & 31u, h = ln >> 5;
-                const uint8_t *k = lds + PIECE * j + 128 * r;
 #pragma unroll
                 for (uint32_t st = 0; st < 4; st++)
-                    s[0] = mma16<float>(*reinterpret_cast<const i4v *>(k + (((2 * st + h) ^ swizzle<C, 1>(r)) << 4)), q[4 * j + st], s[0]);
+                    s[0] = mma16<float>(*reinterpret_cast<const i4v *>(lds + ka[st] + PIECE * j), q[4 * j + st], s[0]);
                 wait_lds();
                 copy(key, DT + j);
             }
@@ -412,13 +427,10 @@ struct WaveAttn<float, D> {
             for (uint32_t j = 0; j < DT; j++) {   // O^T += V^T P^T
                 if (more) wait_copies<4 * (DT - 1)>();
                 else wait_copies<0>();
-                uint8_t *v = lds + PIECE * j;
-                if (decltype(masked)::value) dropped |= drop_not_finite<float, 4>(v, lane);
-                const uint32_t ln = opaque(lane) & 63u, d = ln & 31u, h = ln >> 5;
+                if (decltype(masked)::value) dropped |= drop_not_finite<float, 4>(lds + PIECE * j, lane);
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    const uint32_t r = 8 * (i / 4) + 4 * h + i % 4;
-                    const float a = *reinterpret_cast<const float *>(v + 128 * r + (((d >> 2) ^ swizzle<C, 2>(r)) << 4) + 4 * (d & 3u));
+                    const float a = *reinterpret_cast<const float *>(lds + va[i % 4 / 2] + PIECE * j + 128 * (8 * (i / 4) + i % 4));
                     o[j] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, s[0][i], o[j], 0, 0, 0);
                 }
                 wait_lds();
