@@ -90,18 +90,23 @@ inline PrefixPlan prefix_plan(uint32_t prefix_len, uint32_t tail_cap, uint32_t n
     p.p_slots = elem == 2 && slots > kAttnTileRows ? 128u : kAttnTileRows;
     p.p_tiles = (uint32_t)((slots + p.p_slots - 1) / p.p_slots);
     p.t_tiles = (uint32_t)((n_tokens * group + kAttnTileRows - 1) / kAttnTileRows);
-    // enough chunks for two workgroups a CU, none below 256 keys (two tiles of every wave)
-    auto split = [&](uint32_t keys, uint64_t per_chunk, uint32_t *chunk, uint32_t *n) {
+    // Enough chunks for two workgroups a CU, none below 256 keys (two subtiles of every wave): the tails' fill up to
+    // one a CU, the prefix' the rest, so that the two, which are bound by different things, run side by side (64
+    // sequences of up to 1024 rows behind 32768, bf16: 87 us with two of the prefix a CU, 70 so; 16 of up to 300
+    // behind 8192, f32: 46 and 36).
+    auto split = [&](uint32_t keys, uint64_t per_chunk, uint64_t jobs, uint32_t *chunk, uint32_t *n) {
         if (!keys) return;
-        uint64_t want = (2ull * cus + per_chunk - 1) / per_chunk;
+        uint64_t want = (jobs + per_chunk - 1) / per_chunk;
         const uint64_t most = (keys + 255) / 256;
         if (want > most) want = most;
         if (want > kMaxParts / 2) want = kMaxParts / 2;
         *chunk = (uint32_t)((((uint64_t)keys + want - 1) / want + 127) / 128 * 128);
         *n = (uint32_t)(((uint64_t)keys + *chunk - 1) / *chunk);
     };
-    split(prefix_len, (uint64_t)p.p_tiles * n_kv, &p.p_chunk, &p.n_p);
-    split(tail_cap, (uint64_t)p.t_tiles * n_kv * n_seqs, &p.t_chunk, &p.n_t);
+    const uint64_t per_t = (uint64_t)p.t_tiles * n_kv * n_seqs;
+    split(tail_cap, per_t, (prefix_len ? 1ull : 2ull) * cus, &p.t_chunk, &p.n_t);
+    const uint64_t t_jobs = p.n_t * per_t;
+    split(prefix_len, (uint64_t)p.p_tiles * n_kv, 2ull * cus - (t_jobs < cus ? t_jobs : cus), &p.p_chunk, &p.n_p);
     p.rows = (uint64_t)n_seqs * n_tokens * n_heads;
     p.p_jobs = (uint64_t)p.n_p * p.p_tiles * n_kv;
     p.t_jobs = (uint64_t)p.n_t * p.t_tiles * n_kv * n_seqs;
