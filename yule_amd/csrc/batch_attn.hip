@@ -158,17 +158,23 @@ struct Rows {
     uint32_t stride;
 };
 
-// The scores of N subtiles into probabilities against the new running maximum m of
-// c S (the product and the difference round once, in the fused multiply-add); the
-// weight's sum l (this lane's keys) and the sums o rescaled where it moved.
+// the larger of x and the other half's (lane +- 32)
+__device__ __forceinline__ float max_halves(float x) {
+    const uint32_t u = __float_as_uint(x);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// The running maximum m of c S with N more subtiles of scores; the weight's sum l
+// (this lane's keys) and the sums o rescaled where it moved.
 template <uint32_t N, uint32_t DT>
-__device__ __forceinline__ void online_softmax(f16v (&s)[N], f16v (&o)[DT], float &m, float &l, float c) {
+__device__ __forceinline__ void new_maximum(const f16v (&s)[N], f16v (&o)[DT], float &m, float &l, float c) {
     float cm = s[0][0];
 #pragma unroll
     for (uint32_t n = 0; n < N; n++)
 #pragma unroll
         for (int i = n ? 0 : 1; i < 16; i++) cm = fmaxf(cm, s[n][i]);
-    cm = fmaxf(cm, __shfl_xor(cm, 32, 64)) * c;
+    cm = max_halves(cm) * c;
     if (__ballot(cm > m)) {
         const float mn = fmaxf(m, cm);
         // (m = -inf: nothing was added yet, and the factor multiplies zeros)
@@ -180,14 +186,25 @@ __device__ __forceinline__ void online_softmax(f16v (&s)[N], f16v (&o)[DT], floa
 #pragma unroll
             for (int i = 0; i < 16; i++) o[t][i] *= alpha;
     }
+}
+// scores into weights 2^(c S - m): the product and the difference round once, in the fused multiply-add
+template <uint32_t N>
+__device__ __forceinline__ void weights(f16v (&s)[N], float m, float &l, float c) {
     const float mb = m == -INFINITY ? 0.f : m;   // nothing seen yet: weights of 0
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (uint32_t n = 0; n < N; n++)
 #pragma unroll
         for (int i = 0; i < 16; i++) {
             s[n][i] = __builtin_amdgcn_exp2f(fmaf(s[n][i], c, -mb));
-            l += s[n][i];
+            sum[i % 4] += s[n][i];
         }
+    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+}
+template <uint32_t N, uint32_t DT>
+__device__ __forceinline__ void online_softmax(f16v (&s)[N], f16v (&o)[DT], float &m, float &l, float c) {
+    new_maximum(s, o, m, l, c);
+    weights(s, m, l, c);
 }
 
 // ---- one wave: 32 slots over keys key0, key0 + step, .. < k1 (subtiles of 32)
@@ -552,68 +569,82 @@ struct TileAttn {
             off[0][i] = kc < hb ? r * K.stride + kc : ~0u;
             off[1][i] = vc < hb ? r * V.stride + vc : ~0u;
         }
-        auto copy = [&](uint32_t at, uint32_t buf) {
-            const uint64_t kr = reinterpret_cast<uint64_t>(K.p) + (uint64_t)at * K.stride;
-            const uint64_t vr = reinterpret_cast<uint64_t>(V.p) + (uint64_t)at * V.stride;
-            const uint8_t *kb = uniform(kr), *vb = uniform(vr);
-            const uint32_t dst = lds0 + 2 * TILE * buf;
+        // K's tile at `at` (is_v 0) or V's into half `buf` of the LDS
+        auto copy = [&](uint32_t is_v, uint32_t at, uint32_t buf) {
+            const Rows &R = is_v ? V : K;
+            const uint8_t *base = uniform(reinterpret_cast<uint64_t>(R.p) + (uint64_t)at * R.stride);
+            const uint32_t dst = lds0 + TILE * (2 * buf + is_v);
             if (k1 - at >= KEYS && hb == RB) {
 #pragma unroll
-                for (uint32_t i = 0; i < NC; i++) copy_to_lds(kb, off[0][i], dst + 1024 * i);
-#pragma unroll
-                for (uint32_t i = 0; i < NC; i++) copy_to_lds(vb, off[1][i], dst + TILE + 1024 * i);
+                for (uint32_t i = 0; i < NC; i++) copy_to_lds(base, off[is_v][i], dst + 1024 * i);
             } else if (k1 - at >= KEYS) {
 #pragma unroll
                 for (uint32_t i = 0; i < NC; i++)
-                    if (off[0][i] != ~0u) copy_to_lds(kb, off[0][i], dst + 1024 * i);
-#pragma unroll
-                for (uint32_t i = 0; i < NC; i++)
-                    if (off[1][i] != ~0u) copy_to_lds(vb, off[1][i], dst + TILE + 1024 * i);
+                    if (off[is_v][i] != ~0u) copy_to_lds(base, off[is_v][i], dst + 1024 * i);
             } else {   // rows past the last key repeat it (hidden)
                 const uint32_t last = k1 - at - 1u;
 #pragma unroll
                 for (uint32_t i = 0; i < NC; i++) {
                     const uint32_t L = 64 * (NC * wave + i) + (opaque(lane) & 63u), r = L / C, rr = r < last ? r : last;
-                    const uint32_t kc = 16 * ((L % C) ^ swizzle<C, 1>(r)), vc = 16 * ((L % C) ^ swizzle<C, 2>(r));
-                    if (kc < hb) copy_to_lds(kb, rr * K.stride + kc, dst + 1024 * i);
-                    if (vc < hb) copy_to_lds(vb, rr * V.stride + vc, dst + TILE + 1024 * i);
+                    const uint32_t ch = 16 * ((L % C) ^ (is_v ? swizzle<C, 2>(r) : swizzle<C, 1>(r)));
+                    if (ch < hb) copy_to_lds(base, rr * R.stride + ch, dst + 1024 * i);
                 }
             }
         };
-        copy(k0, 0);
+        // The scores of the next tile are formed while this one's become weights and
+        // meet V: products and vector instructions of one wave overlap then, and not
+        // only those of the two waves of a SIMD.  K is a tile ahead of V for that.
+        copy(0, k0, 0);
+        copy(1, k0, 0);
+        const bool two = k0 + KEYS < k1;
+        if (two) copy(0, k0 + KEYS, 1);
         w.wait_queries();
         uint32_t buf = 0, key = k0;
         bool dropped = false;
-        auto next = [&]() {   // the tile at key is there, the next one on its way
+        f16v s[NSUB];
+        auto scores = [&](uint32_t half) {
+#pragma unroll
+            for (uint32_t n = 0; n < NSUB; n++) s[n] = w.scores(&sh.kv[half][0][n * SUB], lane);
+        };
+        auto meet = [&]() {   // every wave's copies are there, and nobody reads what the next ones replace
+            wait_lds();
+            __builtin_amdgcn_s_barrier();
+            __atomic_signal_fence(__ATOMIC_SEQ_CST);
+        };
+        if (two) wait_copies<2 * NC>();
+        else wait_copies<NC>();
+        meet();
+        if (lim_hi > k0) scores(0);
+        auto next = [&]() {   // this tile's V and the next one's K are there, the ones after them on their way
             wait_copies<0>();
             if (key + KEYS > lim_all)   // (each wave looks at what it copied)
                 dropped |= drop_not_finite<T, NC>(&sh.kv[buf][1][0] + 1024 * NC * wave, lane);
-            wait_lds();
-            __builtin_amdgcn_s_barrier();   // every wave's copies are there, and nobody reads the other half
-            __atomic_signal_fence(__ATOMIC_SEQ_CST);
-            if (key + KEYS < k1) copy(key + KEYS, buf ^ 1u);
+            meet();
+            if (key + 2 * KEYS < k1) copy(0, key + 2 * KEYS, buf);
+            if (key + KEYS < k1) copy(1, key + KEYS, buf ^ 1u);
         };
         for (; key + KEYS <= lim_lo; key += KEYS, buf ^= 1u) {   // tiles that every slot of the wave sees whole
             next();
-            const uint8_t *kt = &sh.kv[buf][0][0], *vt = &sh.kv[buf][1][0];
-            f16v s[NSUB];
+            new_maximum(s, w.o, w.m, w.l, c);
+            f16v p[NSUB];
 #pragma unroll
-            for (uint32_t n = 0; n < NSUB; n++) s[n] = w.scores(kt + n * SUB, lane);
-            online_softmax<NSUB, W::DT>(s, w.o, w.m, w.l, c);
+            for (uint32_t n = 0; n < NSUB; n++) p[n] = s[n];
+            scores(buf ^ 1u);   // (past the last tile: of what the LDS holds, and not looked at)
+            weights(p, w.m, w.l, c);
 #pragma unroll
-            for (uint32_t n = 0; n < NSUB; n++) w.values(s[n], vt + n * SUB, lane);
+            for (uint32_t n = 0; n < NSUB; n++) w.values(p[n], &sh.kv[buf][1][n * SUB], lane);
         }
-        for (; key < k1; key += KEYS, buf ^= 1u) {   // and the others, subtile by subtile
+        for (; key < k1; key += KEYS, buf ^= 1u) {   // and the others
             next();
-#pragma unroll 1
-            for (uint32_t n = 0; n < NSUB; n++) {
-                if (key + 32 * n >= lim_hi) break;
-                const uint32_t ln = opaque(lane) & 63u;
-                f16v s[1] = {w.scores(&sh.kv[buf][0][n * SUB], ln)};
-                W::hide(s[0], key + 32 * n, lim, lane);
-                online_softmax<1, W::DT>(s, w.o, w.m, w.l, c);
-                w.values(s[0], &sh.kv[buf][1][n * SUB], ln);
-            }
+            if (key >= lim_hi) continue;
+#pragma unroll
+            for (uint32_t n = 0; n < NSUB; n++) W::hide(s[n], key + 32 * n, lim, lane);
+            new_maximum(s, w.o, w.m, w.l, c);
+            weights(s, w.m, w.l, c);
+            const uint32_t ln = opaque(lane) & 63u;
+#pragma unroll
+            for (uint32_t n = 0; n < NSUB; n++) w.values(s[n], &sh.kv[buf][1][n * SUB], ln);
+            if (key + KEYS < lim_hi) scores(buf ^ 1u);
         }
         const float l = w.l + __shfl_xor(w.l, 32, 64);
         if (lane == 0) sh.dropped[wave] = dropped;
@@ -757,7 +788,7 @@ struct PrefixArgs {
 // TILE: the prefix by workgroups of 128 slots that share its tiles
 template <typename T, uint32_t D, bool TILE>
 __global__ __launch_bounds__((64 * BlockAttn<T, D>::NW))
-    __attribute__((amdgpu_waves_per_eu(BlockAttn<T, D>::WAVES))) void prefix_attn_kernel(PrefixArgs a) {
+    __attribute__((amdgpu_waves_per_eu(TILE ? (D <= 128 ? 2 : 1) : BlockAttn<T, D>::WAVES))) void prefix_attn_kernel(PrefixArgs a) {
     using B = BlockAttn<T, D>;
     using P = TileAttn<typename std::conditional<TILE, T, _Float16>::type, TILE ? D : 64>;
     __shared__ union {
