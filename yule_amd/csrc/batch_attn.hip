@@ -529,17 +529,21 @@ struct BlockAttn {
 
 // ---- a workgroup of four waves with 32 slots each over tiles of keys that they
 // share (16-bit types): tiles of NSUB subtiles, the next one's K and V on their
-// way into the other half of the LDS while this one is worked on.
-template <typename T, uint32_t D>
+// way into the other half of the LDS while this one is worked on.  KS 2: eight
+// waves, four of which take every other tile, and a join in LDS at the end: half
+// the way through the keys where there are few workgroups.
+template <typename T, uint32_t D, uint32_t KS>
 struct TileAttn {
     using W = WaveAttn<T, D>;
     static constexpr uint32_t NW = 4, NSUB = W::SUB <= 8192 ? 2 : 1, TILE = NSUB * W::SUB, KEYS = 32 * NSUB;
     static constexpr uint32_t NC = NSUB * W::NL / NW;   // copies of a wave per tile of K, and of V
     static_assert(NSUB * W::NL % NW == 0);
     struct Shared {
-        __align__(1024) uint8_t kv[2][2][TILE];
-        uint32_t dropped[NW];
+        __align__(1024) uint8_t kv[KS][2][2][TILE];
+        float m[NW][64], l[NW][64];   // (KS 2)
+        uint32_t dropped[KS * NW];
     };
+    static_assert(KS == 1 || sizeof(Shared::kv) >= NW * 32 * D * 4);
 
     // Keys k0 .. k1 - 1 of the workgroup, every slot of which sees those below
     // lim_all; the wave's slots see keys below lim (each lane's own), all of them
@@ -551,12 +555,14 @@ struct TileAttn {
                                                uint32_t lim_hi, float c, OUT out) {
         constexpr uint32_t RB = W::RB, C = W::C, SUB = W::SUB;
         const uint32_t tid = threadIdx.x, lane = tid & 63u, h = lane >> 5;
-        const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-        const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>((lds_b)&sh.kv[0][0][0]) + 1024 * NC * wave;
+        const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6) % NW, ks = KS > 1 ? __builtin_amdgcn_readfirstlane(tid >> 6) / NW : 0u;
+        auto &kv = sh.kv[ks];
+        const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>((lds_b)&kv[0][0][0]) + 1024 * NC * wave;
         W w;
         w.init(qrow, hb, h);
         if (hb < RB) {   // chunks past the head stay zero: copies leave them out
-            for (uint32_t i = tid; i < 4 * TILE / 16; i += 64 * NW) *reinterpret_cast<i4v *>(&sh.kv[0][0][0] + 16 * i) = i4v{0, 0, 0, 0};
+            for (uint32_t i = tid; i < sizeof(sh.kv) / 16; i += 64 * NW * KS)
+                *reinterpret_cast<i4v *>(&sh.kv[0][0][0][0] + 16 * i) = i4v{0, 0, 0, 0};
             wait_lds();
             __builtin_amdgcn_s_barrier();
         }
@@ -594,36 +600,39 @@ struct TileAttn {
         // The scores of the next tile are formed while this one's become weights and
         // meet V: products and vector instructions of one wave overlap then, and not
         // only those of the two waves of a SIMD.  K is a tile ahead of V for that.
-        copy(0, k0, 0);
-        copy(1, k0, 0);
-        const bool two = k0 + KEYS < k1;
-        if (two) copy(0, k0 + KEYS, 1);
-        w.wait_queries();
-        uint32_t buf = 0, key = k0;
+        constexpr uint32_t STEP = KEYS * KS;
+        uint32_t buf = 0, key = k0 + KEYS * ks;
         bool dropped = false;
         f16v s[NSUB];
         auto scores = [&](uint32_t half) {
 #pragma unroll
-            for (uint32_t n = 0; n < NSUB; n++) s[n] = w.scores(&sh.kv[half][0][n * SUB], lane);
+            for (uint32_t n = 0; n < NSUB; n++) s[n] = w.scores(&kv[half][0][n * SUB], lane);
         };
         auto meet = [&]() {   // every wave's copies are there, and nobody reads what the next ones replace
             wait_lds();
             __builtin_amdgcn_s_barrier();
             __atomic_signal_fence(__ATOMIC_SEQ_CST);
         };
+        if (key < k1) {
+            copy(0, key, 0);
+            copy(1, key, 0);
+        }
+        const bool two = key + STEP < k1;
+        if (two) copy(0, key + STEP, 1);
+        w.wait_queries();
         if (two) wait_copies<2 * NC>();
-        else wait_copies<NC>();
+        else wait_copies<NC>();   // (none at all: nothing to wait for)
         meet();
-        if (lim_hi > k0) scores(0);
+        if (lim_hi > key) scores(0);
         auto next = [&]() {   // this tile's V and the next one's K are there, the ones after them on their way
             wait_copies<0>();
-            if (key + KEYS > lim_all)   // (each wave looks at what it copied)
-                dropped |= drop_not_finite<T, NC>(&sh.kv[buf][1][0] + 1024 * NC * wave, lane);
+            if (key + KEYS > lim_all && key < k1)   // (each wave looks at what it copied)
+                dropped |= drop_not_finite<T, NC>(&kv[buf][1][0] + 1024 * NC * wave, lane);
             meet();
-            if (key + 2 * KEYS < k1) copy(0, key + 2 * KEYS, buf);
-            if (key + KEYS < k1) copy(1, key + KEYS, buf ^ 1u);
+            if (key + 2 * STEP < k1) copy(0, key + 2 * STEP, buf);
+            if (key + STEP < k1) copy(1, key + STEP, buf ^ 1u);
         };
-        for (; key + KEYS <= lim_lo; key += KEYS, buf ^= 1u) {   // tiles that every slot of the wave sees whole
+        for (; key + KEYS <= lim_lo; key += STEP, buf ^= 1u) {   // tiles that every slot of the wave sees whole
             next();
             new_maximum(s, w.o, w.m, w.l, c);
             f16v p[NSUB];
@@ -632,9 +641,10 @@ struct TileAttn {
             scores(buf ^ 1u);   // (past the last tile: of what the LDS holds, and not looked at)
             weights(p, w.m, w.l, c);
 #pragma unroll
-            for (uint32_t n = 0; n < NSUB; n++) w.values(p[n], &sh.kv[buf][1][n * SUB], lane);
+            for (uint32_t n = 0; n < NSUB; n++) w.values(p[n], &kv[buf][1][n * SUB], lane);
         }
-        for (; key < k1; key += KEYS, buf ^= 1u) {   // and the others
+        // and the others; as many meetings for every wave
+        for (; key < k1 + KEYS * ks; key += STEP, buf ^= 1u) {
             next();
             if (key >= lim_hi) continue;
 #pragma unroll
@@ -643,13 +653,42 @@ struct TileAttn {
             weights(s, w.m, w.l, c);
             const uint32_t ln = opaque(lane) & 63u;
 #pragma unroll
-            for (uint32_t n = 0; n < NSUB; n++) w.values(s[n], &sh.kv[buf][1][n * SUB], ln);
-            if (key + KEYS < lim_hi) scores(buf ^ 1u);
+            for (uint32_t n = 0; n < NSUB; n++) w.values(s[n], &kv[buf][1][n * SUB], ln);
+            if (key + STEP < lim_hi) scores(buf ^ 1u);
         }
-        const float l = w.l + __shfl_xor(w.l, 32, 64);
-        if (lane == 0) sh.dropped[wave] = dropped;
+        float l = w.l + __shfl_xor(w.l, 32, 64), M = w.m;
+        if (lane == 0) sh.dropped[NW * ks + wave] = dropped;
         __syncthreads();
-        const uint32_t any = sh.dropped[0] | sh.dropped[1] | sh.dropped[2] | sh.dropped[3];
+        uint32_t any = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < KS * NW; i++) any |= sh.dropped[i];
+        if constexpr (KS > 1) {   // the other waves' sums to the first four, as the lanes hold them
+            f4v *const ob = reinterpret_cast<f4v *>(&sh.kv[0][0][0][0]) + 8 * D * wave + lane;
+            if (ks) {
+                sh.m[wave][lane] = M;
+                sh.l[wave][lane] = l;
+#pragma unroll
+                for (uint32_t t = 0; t < W::DT; t++)
+#pragma unroll
+                    for (uint32_t a = 0; a < 4; a++)
+                        ob[64 * (4 * t + a)] = f4v{w.o[t][4 * a], w.o[t][4 * a + 1], w.o[t][4 * a + 2], w.o[t][4 * a + 3]};
+            }
+            __syncthreads();
+            if (ks) return;
+            const float m1 = sh.m[wave][lane], l1 = sh.l[wave][lane], mn = fmaxf(M, m1);
+            // (no key of the slot: zeros, and a maximum of -inf)
+            const float f0 = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(M - mn), f1 = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m1 - mn);
+            M = mn;
+            l = l * f0 + l1 * f1;
+#pragma unroll
+            for (uint32_t t = 0; t < W::DT; t++)
+#pragma unroll
+                for (uint32_t a = 0; a < 4; a++) {
+                    const f4v x = ob[64 * (4 * t + a)];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) w.o[t][4 * a + e] = w.o[t][4 * a + e] * f0 + x[e] * f1;
+                }
+        }
 #pragma unroll
         for (uint32_t t = 0; t < W::DT; t++)
 #pragma unroll
@@ -659,7 +698,7 @@ struct TileAttn {
                 // (dropped from the first tile on that some slot of the workgroup does not see whole)
                 if (any && d * W::SZ < hb)
                     o = add_not_finite<T>(o, V.p + d * W::SZ, V.stride, lim_all < k0 ? k0 : lim_all - (lim_all - k0) % KEYS, lim);
-                out(d, o, w.m, l);
+                out(d, o, M, l);
             }
     }
 };
@@ -751,16 +790,16 @@ __global__ __launch_bounds__((64 * BlockAttn<T, D>::NW))
 }
 
 // the same by workgroups of 128 slots
-template <typename T, uint32_t D>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1))) void prompt_tile_kernel(PromptArgs a) {
-    using B = TileAttn<T, D>;
+template <typename T, uint32_t D, uint32_t KS>
+__global__ __launch_bounds__(256 * KS) __attribute__((amdgpu_waves_per_eu(D <= 128 || KS > 1 ? 2 : 1))) void prompt_tile_kernel(PromptArgs a) {
+    using B = TileAttn<T, D, KS>;
     __shared__ typename B::Shared sh;
     const uint32_t kvh = blockIdx.x % a.s.n_kv, lane = threadIdx.x & 63u, g = a.s.group;
     uint32_t row0, len, tile;
     if (!find_tile<128>(a.off, a.n_seqs, a.n_rows, g, blockIdx.x / a.s.n_kv, lane, &row0, &len, &tile)) return;
     const uint32_t hb = a.s.hd * sizeof(T), end = len * g - 1u, slot0 = 128 * tile;
     const uint32_t last = slot0 + 127 < end ? slot0 + 127 : end;   // the workgroup's last slot
-    const uint32_t first_w = slot0 + 32 * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t first_w = slot0 + 32 * (__builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3u);
     const uint32_t last_w = first_w + 31 < last ? first_w + 31 : last, mine = first_w + (lane & 31u) < last ? first_w + (lane & 31u) : last;
     const uint32_t r = mine / g;
     const size_t head = (size_t)(kvh * g + (mine - r * g)) * hb;
@@ -790,7 +829,7 @@ template <typename T, uint32_t D, bool TILE>
 __global__ __launch_bounds__((64 * BlockAttn<T, D>::NW))
     __attribute__((amdgpu_waves_per_eu(TILE ? (D <= 128 ? 2 : 1) : BlockAttn<T, D>::WAVES))) void prefix_attn_kernel(PrefixArgs a) {
     using B = BlockAttn<T, D>;
-    using P = TileAttn<typename std::conditional<TILE, T, _Float16>::type, TILE ? D : 64>;
+    using P = TileAttn<typename std::conditional<TILE, T, _Float16>::type, TILE ? D : 64, 1>;
     __shared__ union {
         typename B::Shared block;
         typename std::conditional<TILE, typename P::Shared, char>::type tile;
@@ -952,14 +991,20 @@ static HeadShape head_shape(uint32_t n_heads, uint32_t n_kv, uint32_t hd) {
     return {n_heads / n_kv, n_kv, hd, (float)(1.44269504088896340736 / sqrt((double)hd))};
 }
 
-static int launch_prompt(hipStream_t s, const PromptArgs &a, uint32_t dtype, uint64_t tiles, bool shared) {
+static int launch_prompt(hipStream_t s, const PromptArgs &a, uint32_t dtype, uint64_t tiles, bool shared, bool split) {
     const dim3 grid((uint32_t)(tiles * a.s.n_kv));
     by_shape(dtype, a.s.hd, [&](auto t, auto d) {
         using T = decltype(t);
         constexpr uint32_t D = decltype(d)::value;
         if constexpr (sizeof(T) == 2) {
             if (shared) {
-                hipLaunchKernelGGL((prompt_tile_kernel<T, D>), grid, dim3(256), 0, s, a);
+                if constexpr (D <= 128) {
+                    if (split) {
+                        hipLaunchKernelGGL((prompt_tile_kernel<T, D, 2>), grid, dim3(512), 0, s, a);
+                        return;
+                    }
+                }
+                hipLaunchKernelGGL((prompt_tile_kernel<T, D, 1>), grid, dim3(256), 0, s, a);
                 return;
             }
         }
@@ -1052,7 +1097,9 @@ int yule_hip_prompt_attn(yule_hip_backend *be, const yule_rows *q, const yule_ro
             return set_error(YULE_ERR_INVALID, "prompt_attn: too many rows for one call");
         const PromptArgs a = {cq.p, ck.p, cv.p, co.p, cq.stride, ck.stride, cv.stride, co.stride,
                               static_cast<const uint32_t *>(off), n_seqs, n_rows, head_shape(n_heads, n_kv_heads, head_dim)};
-        return launch_prompt(be->stream, a, dtype, tiles, shared);
+        const char *fs = getenv("YULE_PROMPT_SPLIT");
+        const bool split = fs ? atoi(fs) != 0 : false;
+        return launch_prompt(be->stream, a, dtype, tiles, shared, split);
     });
 }
 
