@@ -165,8 +165,12 @@ __device__ __forceinline__ float max_halves(float x) {
     return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-// The running maximum m of c S with N more subtiles of scores; the weight's sum l
-// (this lane's keys) and the sums o rescaled where it moved.
+// What weights are taken against: a running maximum m of c S that lags up to kLag
+// behind the true one, so that the weight's sum l (this lane's keys) and the sums o
+// are rescaled a few times and not with every new maximum of any slot (half of
+// the subtiles of a long walk; a sixth of its time).  Weights reach 2^kLag then:
+// no 16-bit type minds, and what is small is kept better.
+constexpr float kLag = 8.f;
 template <uint32_t N, uint32_t DT>
 __device__ __forceinline__ void new_maximum(const f16v (&s)[N], f16v (&o)[DT], float &m, float &l, float c) {
     float cm = s[0][0];
@@ -175,7 +179,7 @@ __device__ __forceinline__ void new_maximum(const f16v (&s)[N], f16v (&o)[DT], f
 #pragma unroll
         for (int i = n ? 0 : 1; i < 16; i++) cm = fmaxf(cm, s[n][i]);
     cm = max_halves(cm) * c;
-    if (__ballot(cm > m)) {
+    if (__ballot(cm > m + kLag)) {
         const float mn = fmaxf(m, cm);
         // (m = -inf: nothing was added yet, and the factor multiplies zeros)
         const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
@@ -239,17 +243,21 @@ struct WaveAttn {
 #pragma unroll
         for (uint32_t s = 0; s < NS; s++) asm volatile("" : "+v"(q[s]));
     }
-    // S^T = K Q^T with K's subtile at k
-    __device__ __forceinline__ f16v scores(const uint8_t *k, uint32_t lane) const {
+    // S^T = K Q^T with K's subtile at k; also(i) after product i
+    template <typename F>
+    __device__ __forceinline__ f16v scores(const uint8_t *k, uint32_t lane, F also) const {
         const uint32_t r = lane & 31u, h = lane >> 5;
         f16v s;
 #pragma unroll
         for (int i = 0; i < 16; i++) s[i] = 0.f;
 #pragma unroll
-        for (uint32_t st = 0; st < NS; st++)
+        for (uint32_t st = 0; st < NS; st++) {
             s = mma16<T>(*reinterpret_cast<const i4v *>(k + r * RB + (((2 * st + h) ^ swizzle<C, 1>(r)) << 4)), q[st], s);
+            also(st);
+        }
         return s;
     }
+    __device__ __forceinline__ f16v scores(const uint8_t *k, uint32_t lane) const { return scores(k, lane, [](uint32_t) {}); }
     // key0: the subtile's first key; the slot sees keys below lim
     __device__ __forceinline__ static void hide(f16v &s, uint32_t key0, uint32_t lim, uint32_t lane) {
 #pragma unroll
@@ -257,8 +265,12 @@ struct WaveAttn {
             if (key0 + 8 * (i / 4) + 4 * (lane >> 5) + i % 4 >= lim) s[i] = -INFINITY;
     }
 
-    // O^T += V^T P^T with V's subtile at v
+    // O^T += V^T P^T with V's subtile at v; also(i) after product i
     __device__ __forceinline__ void values(const f16v &s, const uint8_t *v, uint32_t lane) {
+        values(s, v, lane, [](uint32_t) {});
+    }
+    template <typename F>
+    __device__ __forceinline__ void values(const f16v &s, const uint8_t *v, uint32_t lane, F also) {
         const uint32_t h = lane >> 5;
         {
             // the transposing read gives lane l of 16 column l of the four rows that lanes 4 r .. 4 r + 3 point
@@ -277,6 +289,7 @@ struct WaveAttn {
                         (lds_s4)(lds_b)(v + r1 * RB + ((ch ^ swizzle<C, 2>(r1)) << 4) + sub));
                     const auto a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
                     o[t] = mma16<T>(__builtin_bit_cast(i4v, a), p, o[t]);
+                    also(DT * k + t);
                 }
             }
         }
@@ -624,6 +637,36 @@ struct TileAttn {
         else wait_copies<NC>();   // (none at all: nothing to wait for)
         meet();
         if (lim_hi > key) scores(0);
+        // A whole tile's copies between the products, one after every fourth: the
+        // four waves' copies take the memory unit 500 cycles, which they would
+        // otherwise spend waiting for it right after they have met.
+        static_assert(NSUB * W::NS == 4 * NC && NSUB * 2 * W::DT == 4 * NC);
+        uint32_t steady = hb == RB && k1 >= 2 * STEP + KEYS ? k1 - 2 * STEP - KEYS + 1 : 0u;   // keys below: whole tiles two steps on
+        steady = steady < lim_lo ? steady : lim_lo;
+        for (; key < steady && key + KEYS <= lim_lo && key + KEYS <= lim_all; key += STEP, buf ^= 1u) {
+            wait_copies<0>();
+            meet();
+            const uint8_t *kb = uniform(reinterpret_cast<uint64_t>(K.p) + (uint64_t)(key + 2 * STEP) * K.stride);
+            const uint8_t *vb = uniform(reinterpret_cast<uint64_t>(V.p) + (uint64_t)(key + STEP) * V.stride);
+            const uint32_t kd = lds0 + TILE * (2 * buf), vd = lds0 + TILE * (2 * (buf ^ 1u) + 1);
+            new_maximum(s, w.o, w.m, w.l, c);
+            f16v p[NSUB];
+#pragma unroll
+            for (uint32_t n = 0; n < NSUB; n++) p[n] = s[n];
+#pragma unroll
+            for (uint32_t n = 0; n < NSUB; n++)
+                s[n] = w.scores(&kv[buf ^ 1u][0][n * SUB], lane, [&](uint32_t st) {
+                    const uint32_t i = n * W::NS + st;
+                    if (i % 4 == 1) copy_to_lds(kb, off[0][i / 4], kd + 1024 * (i / 4));
+                });
+            weights(p, w.m, w.l, c);
+#pragma unroll
+            for (uint32_t n = 0; n < NSUB; n++)
+                w.values(p[n], &kv[buf][1][n * SUB], lane, [&](uint32_t x) {
+                    const uint32_t i = n * 2 * W::DT + x;
+                    if (i % 4 == 1) copy_to_lds(vb, off[1][i / 4], vd + 1024 * (i / 4));
+                });
+        }
         auto next = [&]() {   // this tile's V and the next one's K are there, the ones after them on their way
             wait_copies<0>();
             if (key + KEYS > lim_all && key < k1)   // (each wave looks at what it copied)
