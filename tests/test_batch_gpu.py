@@ -179,6 +179,74 @@ def test_prompt_attn_long(hip, dt):
         check(got[r], want[r], bound[r], f"row {r}")
 
 
+# 16-bit prompts by workgroups of 128 pairs: many sequences of every length up to a few tiles, with heads that do and do
+# not fill the kernels' rows, and few long ones (split over two groups of waves); tests/test_batch_plan.py has the shapes'
+# plans
+@pytest.mark.parametrize("dt", [DType.F16, DType.BF16], ids=lambda d: d.name)
+@pytest.mark.parametrize("heads,kv,hd,lens,spare", [
+    (16, 16, 64, [0, 1, 2, 63, 64, 65, 127, 128, 129] + [3] * 60 + [33, 31, 50], 4),
+    (32, 16, 80, [0, 1, 31, 32, 33, 63, 64, 65, 96, 127] + [5] * 60 + [130, 20], 0),
+    (32, 16, 128, [1, 64, 66, 190, 200] + [7] * 65 + [34, 0], 3),
+    (32, 16, 256, [1, 40, 65] + [4] * 67 + [100, 0], 1),
+    (48, 16, 96, [1, 43, 65, 129] + [4] * 67 + [100], 0),
+    (32, 8, 128, [1100], 0),
+    (32, 8, 120, [577, 523], 9),
+    (12, 2, 80, [3000], 0),
+    (64, 16, 40, [1100], 0),
+])
+@pytest.mark.parametrize("fused", [False, True], ids=["apart", "fused"])
+def test_prompt_attn_tiles(hip, dt, heads, kv, hd, lens, spare, fused):
+    n, qd, kvd = sum(lens) + spare, heads * hd, kv * hd
+    say(f"[batch] prompt_attn {dt.name} {heads}/{kv}x{hd}, {len(lens)} sequences, {n} rows, fused {fused}")
+    q, k, v = normal(21, (n, qd), dt, 1.5), normal(22, (n, kvd), dt), normal(23, (n, kvd), dt)
+    before = normal(24, (n, qd), dt)
+    with Dev(hip) as d:
+        out, offs = d.up(before), d.up(np.cumsum([0] + lens).astype(np.uint32))
+        if fused:
+            h, ld = d.up(torch.cat([q, k, v], 1)), qd + 2 * kvd
+            args = (Rows(h, ld), Rows(h, ld, qd), Rows(h, ld, qd + kvd))
+        else:
+            args = (d.up(q), d.up(k), d.up(v))
+        hip.prompt_attn(*args, out, offs, len(lens), n, heads, kv, hd, dt)
+        got = d.down(out, (n, qd), dt)
+        hip.prompt_attn(*args, out, offs, len(lens), n, heads, kv, hd, dt)
+        assert torch.equal(bits_of(got), bits_of(d.down(out, (n, qd), dt))), "not the same twice"
+    total = sum(lens)
+    assert torch.equal(bits_of(got[total:]), bits_of(before[total:]))
+    assert torch.isfinite(got[:total].float()).all()
+    # rows: every sequence's last, and some of the longer ones' around the tiles
+    rows, at = set(), 0
+    for m in lens:
+        rows |= {at + r for r in (0, 15, 16, 31, 32, 33, 63, 64, 65, 100, 127, 128, m // 2, m - 1) if 0 <= r < m and (m > 8 or r == m - 1)}
+        at += m
+    rows = sorted(rows)[::max(1, len(rows) * heads // 2500)]
+    want, bound = prompt_reference(q, k, v, lens, heads, kv, hd, dt, set(rows))
+    check(got[rows], want[rows], bound[rows], "prompt_attn")
+
+
+@pytest.mark.parametrize("dt", [DType.F16, DType.BF16], ids=lambda d: d.name)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("heads,kv,hd,lens", [(16, 16, 64, [150, 70] + [1] * 80), (32, 8, 128, [1100])])
+def test_prompt_attn_tiles_hidden_not_finite(hip, dt, bad, heads, kv, hd, lens):
+    say(f"[batch] prompt_attn {dt.name} {heads}/{kv}x{hd}, {bad} in hidden rows of shared tiles")
+    n, at = sum(lens), 101   # of the first sequence
+    q, k, v = (normal(25 + i, (n, w * hd), dt) for i, w in enumerate((heads, kv, kv)))
+    rows = {0, 30, 63, 64, 90, 99, 100, lens[0] + 5 if len(lens) > 1 else 10}
+    want, bound = prompt_reference(q, k, v, lens, heads, kv, hd, dt, rows)
+    v[at], k[at + 3] = bad, bad
+    if len(lens) > 1:
+        v[lens[0] - 1], v[lens[0] + 60] = bad, bad
+    with Dev(hip) as d:
+        out = d.new(q.numel() * 2)
+        hip.prompt_attn(d.up(q), d.up(k), d.up(v), out, d.up(np.cumsum([0] + lens).astype(np.uint32)), len(lens), n, heads, kv, hd, dt)
+        got = d.down(out, tuple(q.shape), dt)
+    rows = sorted(rows)
+    check(got[rows], want[rows], bound[rows], "rows that do not see them")
+    seen = got[at:at + 3].float()
+    assert (seen == bad).all() if bad == bad else torch.isnan(seen).all()
+    assert not torch.isfinite(got[lens[0] - 1].float()).any()
+
+
 @pytest.mark.parametrize("dt", list(TYPES), ids=lambda d: d.name)
 @pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
 def test_prompt_attn_hidden_not_finite(hip, dt, bad):

@@ -46,6 +46,30 @@ int main() {
         CHECK(d4 >= hd && d4 % 32 == 0 && d4 - hd < 32);   // f32: some of the head in every piece of 32 dims
         CHECK(d2 >= hd && (d2 == 64 || d2 == 96 || d2 == 128 || d2 == 256));
     }
+    // prompts: the tiles of any split into sequences fit, and the shapes of the GPU tests take the kernel they are for
+    for (int i = 0; i < 20000; i++) {
+        const uint32_t kv = 1 + (i * 7919u >> 3) % 16, group = 1 + (i * 104729u >> 4) % 16, hd = 8 * (1 + i % 32);
+        const uint32_t seqs = 1 + (i * 31u) % 100;
+        uint64_t rows = 0, tiles32 = 0, tiles128 = 0;
+        for (uint32_t s = 0; s < seqs; s++) {
+            const uint32_t n = (i * 13u + s * 977u) % 1500;
+            rows += n;
+            tiles32 += ((uint64_t)n * group + 31) / 32;
+            tiles128 += ((uint64_t)n * group + 127) / 128;
+        }
+        for (uint32_t elem = 2; elem <= 4; elem += 2) {
+            const PromptPlan p = prompt_plan(seqs, (uint32_t)rows, kv * group, kv, hd, elem, 256);
+            CHECK((p.slots == 32 && p.tiles >= tiles32) || (p.slots == 128 && p.tiles >= tiles128));
+            CHECK(p.split == 1 || (p.split == 2 && p.slots == 128 && hd <= 128));
+            CHECK(elem == 2 || p.slots == 32);
+        }
+    }
+    CHECK(attn_block_room(64, 2) == 4 && attn_block_room(80, 2) == 3 && attn_block_room(128, 2) == 2 && attn_block_room(256, 2) == 1);
+    CHECK(prompt_plan(2, 24, 8, 1, 64, 2, 256).slots == 32);
+    CHECK(prompt_plan(72, 1000, 16, 16, 64, 2, 256).slots == 128 && prompt_plan(72, 1000, 16, 16, 64, 2, 256).split == 1);
+    CHECK(prompt_plan(72, 1000, 32, 16, 256, 2, 256).slots == 128 && prompt_plan(72, 1000, 32, 16, 80, 2, 256).slots == 128);
+    CHECK(prompt_plan(1, 1100, 32, 8, 128, 2, 256).split == 2 && prompt_plan(2, 1100, 32, 8, 128, 2, 256).split == 2);
+    CHECK(prompt_plan(1, 1100, 64, 16, 40, 2, 256).split == 1);
     // plans: chunks cover the keys once, jobs fit, results lie in the workspace
     unsigned seed = 1;
     auto rnd = [&](uint32_t n) { seed = seed * 1664525u + 1013904223u; return (seed >> 8) % n; };

@@ -791,12 +791,13 @@ __device__ __forceinline__ bool find_tile(const uint32_t *off, uint32_t n_seqs, 
             e = e > b ? e : b;
         }
         const uint32_t mine = ((e - b) * group + SLOTS - 1) / SLOTS;
-        uint32_t sum = mine;
-#pragma unroll
-        for (uint32_t d = 1; d < 64; d *= 2) {
-            const uint32_t x = __shfl_up(sum, d, 64);
-            if (lane >= d) sum += x;
-        }
+        uint32_t sum = mine;   // inclusive over the lanes, by DPP row shifts and row broadcasts
+        sum += __builtin_amdgcn_update_dpp(0, (int)sum, 0x111, 0xf, 0xf, false);
+        sum += __builtin_amdgcn_update_dpp(0, (int)sum, 0x112, 0xf, 0xf, false);
+        sum += __builtin_amdgcn_update_dpp(0, (int)sum, 0x114, 0xf, 0xf, false);
+        sum += __builtin_amdgcn_update_dpp(0, (int)sum, 0x118, 0xf, 0xf, false);
+        sum += __builtin_amdgcn_update_dpp(0, (int)sum, 0x142, 0xa, 0xf, false);
+        sum += __builtin_amdgcn_update_dpp(0, (int)sum, 0x143, 0xc, 0xf, false);
         const uint64_t here = __ballot(before + sum > y);
         if (here) {
             const int at = __builtin_ctzll(here);
@@ -1034,15 +1035,15 @@ static HeadShape head_shape(uint32_t n_heads, uint32_t n_kv, uint32_t hd) {
     return {n_heads / n_kv, n_kv, hd, (float)(1.44269504088896340736 / sqrt((double)hd))};
 }
 
-static int launch_prompt(hipStream_t s, const PromptArgs &a, uint32_t dtype, uint64_t tiles, bool shared, bool split) {
-    const dim3 grid((uint32_t)(tiles * a.s.n_kv));
+static int launch_prompt(hipStream_t s, const PromptArgs &a, uint32_t dtype, const PromptPlan &p) {
+    const dim3 grid((uint32_t)(p.tiles * a.s.n_kv));
     by_shape(dtype, a.s.hd, [&](auto t, auto d) {
         using T = decltype(t);
         constexpr uint32_t D = decltype(d)::value;
         if constexpr (sizeof(T) == 2) {
-            if (shared) {
+            if (p.slots == 128) {
                 if constexpr (D <= 128) {
-                    if (split) {
+                    if (p.split == 2) {
                         hipLaunchKernelGGL((prompt_tile_kernel<T, D, 2>), grid, dim3(512), 0, s, a);
                         return;
                     }
@@ -1131,18 +1132,12 @@ int yule_hip_prompt_attn(yule_hip_backend *be, const yule_rows *q, const yule_ro
         if (out->buffer == q->buffer || out->buffer == k->buffer || out->buffer == v->buffer || out->buffer == offsets)
             return set_error(YULE_ERR_INVALID, "prompt_attn: an input and the output alias");
         if (!n_seqs || !n_rows) return YULE_OK;
-        // tiles of all sequences: each has at most one that is not full
-        const uint64_t group = n_heads / n_kv_heads;
-        const char *force = getenv("YULE_PROMPT_TILE");
-        const bool shared = elem == 2 && (force ? atoi(force) != 0 : true);
-        const uint64_t tiles = n_rows * group / (shared ? 128 : kAttnTileRows) + n_seqs;
-        if ((uint64_t)n_rows * group >= (uint64_t)1 << 31 || tiles * n_kv_heads > kMaxWorkgroups)
+        const PromptPlan p = prompt_plan(n_seqs, n_rows, n_heads, n_kv_heads, head_dim, elem, (uint32_t)be->props.multiProcessorCount);
+        if ((uint64_t)n_rows * (n_heads / n_kv_heads) >= (uint64_t)1 << 31 || p.tiles * n_kv_heads > kMaxWorkgroups)
             return set_error(YULE_ERR_INVALID, "prompt_attn: too many rows for one call");
         const PromptArgs a = {cq.p, ck.p, cv.p, co.p, cq.stride, ck.stride, cv.stride, co.stride,
                               static_cast<const uint32_t *>(off), n_seqs, n_rows, head_shape(n_heads, n_kv_heads, head_dim)};
-        const char *fs = getenv("YULE_PROMPT_SPLIT");
-        const bool split = fs ? atoi(fs) != 0 : false;
-        return launch_prompt(be->stream, a, dtype, tiles, shared, split);
+        return launch_prompt(be->stream, a, dtype, p);
     });
 }
 

@@ -54,6 +54,36 @@ constexpr uint32_t kAttnTileRows = 32;
 constexpr uint64_t kMaxWorkgroups = (uint64_t)1 << 23;
 constexpr uint32_t kMaxKeys = 1u << 30;   // of a prefix, and of a tail
 
+// ---- prompt_attn: who takes a tile of (row, head of the group) pairs of a KV head.
+// f32: a workgroup per 32 of them, its four waves share the keys.  16-bit types,
+// by what was measured (MI355X, bf16, us; heads / KV heads x head_dim, rows):
+//   32     the same, while all of them find room on the chip at once: latency
+//          counts, and many small workgroups have the shortest way
+//          (32/8x128: 128 rows 6.8 against 8.9 with 128, 500 rows 11.8 against
+//          14.9; 750 rows, too many, 22.0 against 18.5; 32/4x64, 1000 rows: 14.1
+//          against 15.6 and 17.4)
+//   split  128 a workgroup of eight waves, half of which take every other tile of
+//          keys: few workgroups with a long way (32/8x128: 1000 rows 21.8 against
+//          23.3, 2000 rows 47.1 against 45.8; 12/2x80, 3000 rows: 40.8 against
+//          51.5; seven sequences of 259 rows on average 28.1 against 22.9)
+//   128    four waves of 32 over shared tiles of keys: throughput
+struct PromptPlan {
+    uint32_t slots, split;   // pairs of a tile, groups of waves that share its keys
+    uint64_t tiles;          // at most: each sequence has one that is not full
+};
+// workgroups of the 32-pair kernel that a CU's LDS has room for
+inline uint32_t attn_block_room(uint32_t hd, uint32_t elem) {
+    const uint32_t d = attn_padded_dim(hd, elem), lds = 4 * (elem == 4 ? 128 * d : 64 * d * elem) + 2048;
+    return 163840u / lds;
+}
+inline PromptPlan prompt_plan(uint32_t n_seqs, uint32_t n_rows, uint32_t n_heads, uint32_t n_kv, uint32_t hd,
+                              uint32_t elem, uint32_t cus) {
+    const uint64_t pairs = (uint64_t)n_rows * (n_heads / n_kv), small = pairs / 32 + n_seqs, large = pairs / 128 + n_seqs;
+    if (elem == 4 || small * n_kv <= (uint64_t)attn_block_room(hd, elem) * cus) return {32, 1, small};
+    const bool split = 2 * large * n_kv <= 3ull * cus && n_rows / n_seqs >= 512 && hd <= 128;
+    return {128, split ? 2u : 1u, large};
+}
+
 // ---- verify_drafts: values of a row per workgroup, and what a chunk leaves (the
 // f64 sum of its weights, and the last place that has one)
 constexpr uint32_t kVerifyChunk = 4096, kMaxVocab = 1u << 30, kMaxDrafts = 1024;
