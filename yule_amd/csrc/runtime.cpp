@@ -172,8 +172,8 @@ int yule_hip_create(int device, yule_hip_backend **out) {
     }
     if ((rc = hip_error(hipMalloc(&be->argmax_ws, argmax_ws_bytes()), "create: argmax workspace")) ||
         (rc = hip_error(hipMemsetAsync(be->argmax_ws, 0, argmax_ws_bytes(), be->stream), "create: argmax workspace")) ||
-        (rc = hip_error(hipMalloc(&be->verify_ws, kVerifyTickets * 4), "create: verify tickets")) ||
-        (rc = hip_error(hipMemsetAsync(be->verify_ws, 0, kVerifyTickets * 4, be->stream), "create: verify tickets"))) {
+        (rc = hip_error(hipMalloc(&be->verify_ws, kVerifyTickets * kVerifyTicketWords * 4), "create: verify tickets")) ||
+        (rc = hip_error(hipMemsetAsync(be->verify_ws, 0, kVerifyTickets * kVerifyTicketWords * 4, be->stream), "create: verify tickets"))) {
         yule_hip_destroy(be);
         return rc;
     }

@@ -10,9 +10,13 @@
 //
 // One row of p and one of q is all that has to be read (the drafts' own
 // probabilities besides): bandwidth for a batch, latency for a single request.
-// One launch: the rows are cut into chunks of 4096 values, a workgroup each,
-// which leave their sums; the workgroup that takes a sequence's last ticket finds
-// the chunk that the pick falls into and walks that one again.
+// One launch: the rows are cut into chunks of 4096 values, a workgroup each, which
+// leave their sums; the one that takes a sequence's last ticket finds the chunk that
+// the pick falls into and loads that one again.  (A workgroup of 1024 threads for a
+// whole row of 32000 values needs no tickets, but is no faster up to 64 sequences:
+// 7.4 against 7.0 us for one, 10.4 against 10.6 for 64; 200: 12.1 against 16.2.)
+// A row of one chunk takes 4.9 us; a ticket, the sums and the chunk once more add
+// 2, and 64 requests of 32000 values, 16 MB, 10.6 in all.
 #include <type_traits>
 
 #include "batch_plan.h"
@@ -28,8 +32,8 @@ struct VerifyArgs {
     const uint32_t *lens;        // drafts of each sequence, or null
     uint32_t *accepted, *tokens; // [n_seqs], [n_seqs][n_draft + 1]
     uint32_t n_draft, vocab, chunks, seq0;
-    VerifySum *sums;             // [sequences of the launch][chunks]
-    uint32_t *tickets;           // [sequences of the launch], zero before and after
+    double *sums;                // [sequences of the launch][chunks]
+    uint32_t *tickets;           // one of kVerifyTicketWords for each sequence of the launch, zero before and after
 };
 
 // a weight: what is not a positive number counts as nothing
@@ -81,49 +85,31 @@ __device__ __forceinline__ double wave_scan(double x) {
     step(integral_constant<int, 0x143>{}, integral_constant<int, 0xc>{});
     return x;
 }
-__device__ __forceinline__ double last_lane(double x) {
+__device__ __forceinline__ double lane_of(double x, uint32_t l) {
     const uint64_t b = __builtin_bit_cast(uint64_t, x);
-    return __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(b >> 32), 63) << 32 |
-                                          (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, 63));
-}
-__device__ __forceinline__ int wave_max(int x) {
-#pragma unroll
-    for (int d = 32; d; d /= 2) {
-        const int y = __shfl_xor(x, d, 64);
-        x = x > y ? x : y;
-    }
-    return x;
+    return __builtin_bit_cast(double, (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(b >> 32), (int)l) << 32 |
+                                          (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, (int)l));
 }
 
-// Values x0 + 1024 j + 4 tid + e (j, e < 4) of a row in this thread's registers,
-// 0 past n: 16-byte loads where the row allows them.
-__device__ __forceinline__ void load_chunk(const float *row, uint32_t x0, uint32_t n, uint32_t tid, float v[4][4]) {
-    const bool whole = x0 + kVerifyChunk <= n && (reinterpret_cast<uintptr_t>(row) & 15u) == 0;
-    if (whole) {
-#pragma unroll
-        for (uint32_t j = 0; j < 4; j++) {
-            const float4 f = *reinterpret_cast<const float4 *>(row + x0 + 1024 * j + 4 * tid);
-            v[j][0] = f.x, v[j][1] = f.y, v[j][2] = f.z, v[j][3] = f.w;
-        }
+// values x .. x + 3 of a row of n, 0 past its end: one load where the row allows it
+__device__ __forceinline__ void load4(const float *row, uint32_t x, uint32_t n, bool aligned, float v[4]) {
+    if (aligned && x + 4 <= n) {
+        const float4 f = *reinterpret_cast<const float4 *>(row + x);
+        v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
     } else {
 #pragma unroll
-        for (uint32_t j = 0; j < 4; j++)
-#pragma unroll
-            for (uint32_t e = 0; e < 4; e++) {
-                const uint32_t x = x0 + 1024 * j + 4 * tid + e;
-                const float f = row[x < n ? x : n - 1u];
-                v[j][e] = x < n ? f : 0.f;
-            }
+        for (uint32_t e = 0; e < 4; e++) v[e] = x + e < n ? row[x + e] : 0.f;
     }
 }
 
-// A workgroup per chunk; the one that takes its sequence's last ticket picks and
-// answers.  Sums are taken in one order, whoever is last.
+// A thread has 4 J values of a chunk, 4 NT j + 4 tid .., so a wave's are 256 in a row
+// (a group), NG groups a chunk.  Sums are taken in one order, whoever takes the
+// last ticket.
 __global__ __launch_bounds__(256) void verify_kernel(VerifyArgs a) {
-    __shared__ double part[16];   // sums of 256 weights each: 1024 j + 256 wave ..
-    __shared__ int lasts[4];      // last places that have a weight, by wave
-    __shared__ double target, before;
-    __shared__ uint32_t is_last, at, token, again;
+    constexpr uint32_t NT = 256, J = 4, NW = NT / 64, NG = NW * J, CHUNK = kVerifyChunk;
+    static_assert(CHUNK == 4 * NT * J && NG <= 64);
+    __shared__ double part[NG];   // the groups' sums
+    __shared__ uint32_t shared_last, token;
     const uint32_t s = blockIdx.x / a.chunks, chunk = blockIdx.x % a.chunks, seq = a.seq0 + s;
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
     uint32_t count;
@@ -131,180 +117,128 @@ __global__ __launch_bounds__(256) void verify_kernel(VerifyArgs a) {
     const float *p, *q;
     rows_of(a, seq, n, count, &p, &q);
 
-    double w[4][4];   // this thread's weights of a chunk
-    auto weigh = [&](uint32_t c) {
-        float pv[4][4], qv[4][4];
-        load_chunk(p, c * kVerifyChunk, a.vocab, tid, pv);
-        if (q) load_chunk(q, c * kVerifyChunk, a.vocab, tid, qv);
+    float pv[J][4], qv[J][4];   // this thread's values of a chunk
+    auto four = [&](uint32_t j, double w[4]) {
 #pragma unroll
-        for (uint32_t j = 0; j < 4; j++) {
+        for (uint32_t e = 0; e < 4; e++) w[e] = weight(q ? (double)pv[j][e] - (double)qv[j][e] : (double)pv[j][e]);
+        return (w[0] + w[1]) + (w[2] + w[3]);
+    };
+    double group, upto;         // lane's group (of the first NG lanes), and the sum up to and with it
+    auto weigh = [&](uint32_t c) {   // the chunk's sum (in every lane)
+        const bool p_al = (reinterpret_cast<uintptr_t>(p) & 15u) == 0, q_al = (reinterpret_cast<uintptr_t>(q) & 15u) == 0;
 #pragma unroll
-            for (uint32_t e = 0; e < 4; e++) w[j][e] = weight(q ? (double)pv[j][e] - (double)qv[j][e] : (double)pv[j][e]);
-            const double sum = last_lane(wave_scan((w[j][0] + w[j][1]) + (w[j][2] + w[j][3])));
-            if (lane == 0) part[4 * j + wave] = sum;
+        for (uint32_t j = 0; j < J; j++) load4(p, c * CHUNK + 4 * NT * j + 4 * tid, a.vocab, p_al, pv[j]);
+        if (q) {
+#pragma unroll
+            for (uint32_t j = 0; j < J; j++) load4(q, c * CHUNK + 4 * NT * j + 4 * tid, a.vocab, q_al, qv[j]);
         }
-        int last = -1;
 #pragma unroll
-        for (uint32_t j = 0; j < 4; j++)
-#pragma unroll
-            for (uint32_t e = 0; e < 4; e++)
-                if (w[j][e] > 0.0) last = (int)(c * kVerifyChunk + 1024 * j + 4 * tid + e);
-        last = wave_max(last);
-        if (lane == 0) lasts[wave] = last;
+        for (uint32_t j = 0; j < J; j++) {
+            double w[4];
+            const double sum = wave_scan(four(j, w));
+            if (lane == 63) part[NW * j + wave] = sum;
+        }
         __syncthreads();
+        group = lane < NG ? part[lane] : 0.0;
+        upto = wave_scan(group);
+        return lane_of(upto, 63);
     };
-    // (every thread) the chunk that was weighed
-    auto chunk_sum = [&](int *last) {
-        double sum = 0.0;
-#pragma unroll
-        for (uint32_t i = 0; i < 16; i++) sum += part[i];
-        *last = -1;
-#pragma unroll
-        for (uint32_t i = 0; i < 4; i++) *last = lasts[i] > *last ? lasts[i] : *last;
-        return sum;
-    };
-    auto put = [&](uint32_t c, double sum, int last) {   // (one lane)
-        uint64_t *o = reinterpret_cast<uint64_t *>(a.sums + (size_t)s * a.chunks + c);
-        __hip_atomic_store(o, __builtin_bit_cast(uint64_t, sum), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        __hip_atomic_store(o + 1, (uint64_t)(int64_t)last, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    auto put = [&](uint32_t c, double sum) {   // (one lane) complete at device scope when it returns, without a cache-wide fence
+        __hip_atomic_store(reinterpret_cast<uint64_t *>(a.sums + (size_t)s * a.chunks + c), __builtin_bit_cast(uint64_t, sum),
+                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        __atomic_signal_fence(__ATOMIC_SEQ_CST);
+        __builtin_amdgcn_s_waitcnt(0);
+        __atomic_signal_fence(__ATOMIC_SEQ_CST);
     };
 
-    weigh(chunk);
-    if (wave == 0) {
-        uint32_t mine = 1;
-        int last;
-        const double sum = chunk_sum(&last);
-        if (a.chunks > 1) {
-            if (lane == 0) {
-                // complete at device scope before the ticket is taken (no cache-wide fence)
-                put(chunk, sum, last);
-                __atomic_signal_fence(__ATOMIC_SEQ_CST);
-                __builtin_amdgcn_s_waitcnt(0);
-                __atomic_signal_fence(__ATOMIC_SEQ_CST);
-                mine = __hip_atomic_fetch_add(a.tickets + s, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.chunks - 1u;
-                if (mine) __hip_atomic_store(a.tickets + s, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            }
-            mine = __builtin_amdgcn_readfirstlane(mine);
+    double all = weigh(chunk), before = 0.0;
+    uint32_t at = 0;
+    if (a.chunks > 1) {
+        if (tid == 0) {
+            put(chunk, all);
+            uint32_t *ticket = a.tickets + kVerifyTicketWords * s;
+            const bool mine = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == a.chunks - 1u;
+            if (mine) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            shared_last = mine;
         }
-        if (lane == 0) is_last = mine;
+        __syncthreads();
+        if (!shared_last) return;
     }
-    __syncthreads();
-    if (!is_last) return;
-
-    for (;;) {
-        // the chunk that the pick falls into, 64 chunks at a time
-        if (wave == 0) {
-            __atomic_signal_fence(__ATOMIC_SEQ_CST);
-            double c_sum;   // lane's chunk (without others this one)
-            int c_last;
-            auto load_sums = [&](uint32_t c) {
-                int last;
-                const double sum = chunk_sum(&last);
-                c_sum = c == 0 ? sum : 0.0;
-                c_last = c == 0 ? last : -1;
-                if (a.chunks > 1) {
-                    c_sum = 0.0, c_last = -1;
-                    if (c < a.chunks) {
-                        const uint64_t *o = reinterpret_cast<const uint64_t *>(a.sums + (size_t)s * a.chunks + c);
-                        c_sum = __builtin_bit_cast(double, __hip_atomic_load(o, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
-                        c_last = (int)__hip_atomic_load(o + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                    }
-                }
-            };
-            double all = 0.0;
-            int last = -1;
-            for (uint32_t c0 = 0; c0 < a.chunks; c0 += 64) {
-                load_sums(c0 + lane);
-                all += last_lane(wave_scan(c_sum));
-                const int l = wave_max(c_last);
-                last = l > last ? l : last;
-            }
-            const double t = (double)a.u[(size_t)seq * (a.n_draft + 1) + a.n_draft] * all;
+    const double u = a.u[(size_t)seq * (a.n_draft + 1) + a.n_draft];
+    double target;
+    for (;;) {   // (twice if max(p - q, 0) is zero everywhere)
+        if (a.chunks > 1) {   // every wave for itself: all the sums, then the chunk that the target falls into
             double sum = 0.0;
-            uint32_t hit = a.chunks;
+            auto sum_of = [&](uint32_t c) {
+                return c < a.chunks ? __builtin_bit_cast(double, __hip_atomic_load(reinterpret_cast<uint64_t *>(a.sums + (size_t)s * a.chunks + c),
+                                                                                   __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT))
+                                    : 0.0;
+            };
+            const double first = sum_of(lane);
+            all = lane_of(wave_scan(first), 63);
+            for (uint32_t c0 = 64; c0 < a.chunks; c0 += 64) all += lane_of(wave_scan(sum_of(c0 + lane)), 63);
+            target = u * all;
+            at = 0;
             for (uint32_t c0 = 0; c0 < a.chunks; c0 += 64) {
-                if (a.chunks > 64) load_sums(c0 + lane);
-                const double upto = wave_scan(c_sum);
-                const uint64_t past = __ballot(c0 + lane < a.chunks && sum + upto > t);
-                if (past) {
-                    const int l = __builtin_ctzll(past);
-                    hit = c0 + (uint32_t)l;
-                    const double up = __shfl(upto, l ? l - 1 : 0, 64);
-                    if (l) sum += up;
-                    break;
+                const double mine = c0 ? sum_of(c0 + lane) : first, up = wave_scan(mine);
+                const uint64_t some = __ballot(mine > 0.0), past = __ballot(mine > 0.0 && sum + up > target);
+                if (some) {   // the first past it, or so far the last that has a weight (u, or a rounding, at the very end)
+                    const uint32_t l = past ? (uint32_t)__builtin_ctzll(past) : 63u - (uint32_t)__builtin_clzll(some);
+                    at = c0 + l;
+                    before = l ? sum + lane_of(up, l - 1u) : sum;
                 }
-                sum += last_lane(upto);
+                if (past) break;
+                sum += lane_of(up, 63);
             }
-            if (lane == 0) {
-                // not passed at all (u, or a rounding, at the very end): the last token that has a weight, if one has
-                token = last < 0 ? YULE_NO_TOKEN : (uint32_t)last;
-                target = t, before = sum, at = hit;
-                again = last < 0 && q;
-            }
+        } else {
+            target = u * all;
         }
-        __syncthreads();
-        if (!again) break;
+        if (all > 0.0 || !q) break;
         // p = q at a draft that is not kept (roundings can leave that, or a draft that is no token): p itself
         q = nullptr;
+        __syncthreads();   // (part has been read)
         for (uint32_t c = 0; c < a.chunks; c++) {
-            weigh(c);
-            if (tid == 0 && a.chunks > 1) {
-                int last;
-                const double sum = chunk_sum(&last);
-                put(c, sum, last);
-            }
-            if (c + 1 < a.chunks) __syncthreads();
+            all = weigh(c);
+            if (tid == 0 && a.chunks > 1) put(c, all);
+            __syncthreads();
         }
-        if (tid == 0) {   // (read by the first wave only, which waits for them here)
-            __atomic_signal_fence(__ATOMIC_SEQ_CST);
-            __builtin_amdgcn_s_waitcnt(0);
-            __atomic_signal_fence(__ATOMIC_SEQ_CST);
-        }
-        __syncthreads();
     }
-    if (at < a.chunks) {
-        if (a.chunks > 1) weigh(at);   // (one chunk: still there)
-        // The 256 values, then the four, then the value.  (Sums taken in other orders may round to either side of the
-        // target: then the last with a weight.)
-        double run = before, sum = before;
-        uint32_t i = 0;
-        for (uint32_t k = 0; k < 16; k++) {
-            if (part[k] > 0.0) {
-                i = k;
-                sum = run;
-                if (run + part[k] > target) break;
-            }
-            run += part[k];
-        }
-        if (wave == (i & 3u)) {
-            double mine[4];
+    if (a.chunks > 1) {
+        __syncthreads();
+        (void)weigh(at);
+    }
+    // The group, then the four, then the value: the first that passes the target, or (sums taken in other orders may
+    // round to either side of it) the last that has a weight.
+    if (tid == 0) token = YULE_NO_TOKEN;   // nothing has a weight
+    {
+        const uint64_t some = __ballot(group > 0.0), past = __ballot(group > 0.0 && before + upto > target);
+        const uint32_t i = past ? (uint32_t)__builtin_ctzll(past) : some ? 63u - (uint32_t)__builtin_clzll(some) : 0u;
+        const double sum = i ? before + lane_of(upto, i - 1u) : before;
+        __syncthreads();
+        if (some && wave == i % NW) {
+            double w[4] = {0.0, 0.0, 0.0, 0.0}, here = 0.0;
 #pragma unroll
-            for (uint32_t j = 0; j < 4; j++)
-                if (j == i >> 2) {
-#pragma unroll
-                    for (uint32_t e = 0; e < 4; e++) mine[e] = w[j][e];
-                }
-            const double four = (mine[0] + mine[1]) + (mine[2] + mine[3]);
-            const double upto = sum + wave_scan(four);
-            const uint64_t past = __ballot(upto > target && four > 0.0), some = __ballot(four > 0.0);
-            const uint32_t l = past ? (uint32_t)__builtin_ctzll(past) : some ? 63u - (uint32_t)__builtin_clzll(some) : 0u;
-            double here = __shfl_up(upto, 1, 64);
-            if (lane == 0) here = sum;
-            if (lane == l && some) {
+            for (uint32_t j = 0; j < J; j++)
+                if (j == i / NW) here = four(j, w);
+            const double up = sum + wave_scan(here);
+            const uint64_t any = __ballot(here > 0.0), over = __ballot(here > 0.0 && up > target);
+            const uint32_t m = over ? (uint32_t)__builtin_ctzll(over) : any ? 63u - (uint32_t)__builtin_clzll(any) : 0u;
+            double r = m ? lane_of(up, m - 1u) : sum;
+            if (lane == m && any) {
                 uint32_t pick = 0;
-                bool found = false;
+                bool got = false;
 #pragma unroll
                 for (uint32_t e = 0; e < 4; e++) {
-                    here += mine[e];
-                    if (mine[e] > 0.0 && !found) pick = e;
-                    found = found || here > target;
+                    r += w[e];
+                    if (w[e] > 0.0 && !got) pick = e;
+                    got = got || (w[e] > 0.0 && r > target);
                 }
-                token = at * kVerifyChunk + 1024 * (i >> 2) + 4 * tid + pick;
+                token = at * CHUNK + 4 * NT * (i / NW) + 4 * tid + pick;
             }
         }
     }
     __syncthreads();
-    for (uint32_t i = tid; i <= a.n_draft; i += 256)
+    for (uint32_t i = tid; i <= a.n_draft; i += NT)
         a.tokens[(size_t)seq * (a.n_draft + 1) + i] = i < n    ? a.drafts[(size_t)seq * a.n_draft + i]
                                                       : i == n ? token
                                                                : YULE_NO_TOKEN;
@@ -342,14 +276,14 @@ extern "C" int yule_hip_verify_drafts(yule_hip_backend *be, const yule_rows *tar
         const uint64_t chunks = (vocab + kVerifyChunk - 1) / kVerifyChunk;
         if ((uint64_t)n_seqs * chunks > kMaxWorkgroups) return set_error(YULE_ERR_INVALID, "verify_drafts: too many rows for one call");
         ScratchLease ws;   // held until the launches are enqueued
-        if ((rc = get_scratch(be, (n_seqs < kVerifyTickets ? n_seqs : kVerifyTickets) * chunks * sizeof(VerifySum), &ws))) return rc;
+        if ((rc = get_scratch(be, (n_seqs < kVerifyTickets ? n_seqs : kVerifyTickets) * chunks * sizeof(double), &ws))) return rc;
         a.p = static_cast<const float *>(pp), a.q = static_cast<const float *>(pq);
         a.ps = target->stride, a.qs = n_draft ? draft->stride : 0;
         a.drafts = static_cast<const uint32_t *>(pd), a.u = static_cast<const float *>(pu);
         a.lens = static_cast<const uint32_t *>(pl);
         a.accepted = static_cast<uint32_t *>(pa), a.tokens = static_cast<uint32_t *>(pt);
         a.n_draft = n_draft, a.vocab = vocab, a.chunks = (uint32_t)chunks;
-        a.sums = static_cast<VerifySum *>(ws.ptr);
+        a.sums = static_cast<double *>(ws.ptr);
         a.tickets = static_cast<uint32_t *>(be->verify_ws);
         for (uint32_t s0 = 0; s0 < n_seqs; s0 += kVerifyTickets) {   // (a ticket each)
             const uint32_t now = n_seqs - s0 < kVerifyTickets ? n_seqs - s0 : kVerifyTickets;
