@@ -316,6 +316,14 @@ PREFIXES = [
     (2, 2, 8, 520, 600, [600, 513, 99, 2 ** 32 - 1], 1),   # more than one chunk of each; a length above the capacity
     (2, 1, 64, 10, 80, [80, 70], 64),
     (2, 2, 152, 90, 20, [20, 7], 2),
+    # (above: mostly one launch for few keys; from here on by chunks)
+    (6, 2, 80, 600, 70, [70, 5, 0, 33], 5),
+    (4, 4, 128, 700, 64, [64, 31], 2),
+    (2, 1, 256, 565, 40, [40, 3], 3),
+    (16, 1, 64, 540, 12, [12, 3, 9, 4, 1], 4),
+    (4, 1, 64, 0, 530, [130, 0, 2, 529], 3),
+    (4, 1, 64, 577, 0, [0, 9], 2),
+    (64, 1, 64, 600, 30, [3, 30], 2),
     (4, 1, 24, 70, 33, [33, 0, 5], 1),
 ]
 
@@ -367,10 +375,11 @@ def test_prefix_attn_many(hip, dt):
 
 @pytest.mark.parametrize("dt", list(TYPES), ids=lambda d: d.name)
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
-def test_prefix_attn_hidden_not_finite(hip, dt, bad):
+@pytest.mark.parametrize("prefix", [50, 600])
+def test_prefix_attn_hidden_not_finite(hip, dt, bad, prefix):
     """Rows of a tail behind its length, another sequence's, and drafts that an earlier token does not see."""
-    heads, kv, hd, prefix, cap, lens, tokens = 4, 2, 64, 50, 40, [30, 40, 8], 4
-    say(f"[batch] prefix_attn {dt.name}, {bad} in hidden rows")
+    heads, kv, hd, cap, lens, tokens = 4, 2, 64, 40, [30, 40, 8], 4
+    say(f"[batch] prefix_attn {dt.name}, prefix {prefix}, {bad} in hidden rows")
     q, kp, vp, kt, vt = prefix_inputs(50, heads, kv, hd, prefix, cap, lens, tokens, dt)
     want, bound = prefix_reference(q, kp, vp, kt, vt, lens, cap, tokens, heads, kv, hd, dt)
     kt[30:40], vt[30:40] = bad, bad                # behind sequence 0
@@ -404,9 +413,10 @@ def test_prefix_attn_far_rows(hip):
 
 
 @pytest.mark.parametrize("dt", list(TYPES), ids=lambda d: d.name)
-def test_prefix_attn_continues_prompt_attn(hip, dt):
+@pytest.mark.parametrize("prefix", [70, 520])
+def test_prefix_attn_continues_prompt_attn(hip, dt, prefix):
     """The newest tokens over prefix and tail are the last rows of the whole sequences as packed prompts."""
-    heads, kv, hd, prefix, cap, lens, tokens = 8, 2, 64, 70, 33, [33, 9, 5], 5
+    heads, kv, hd, cap, lens, tokens = 8, 2, 64, 33, [33, 9, 5], 5
     say(f"[batch] prefix_attn against prompt_attn {dt.name}")
     _, kp, vp, kt, vt = prefix_inputs(70, heads, kv, hd, prefix, cap, lens, tokens, dt)
     whole = [prefix + n for n in lens]
@@ -593,7 +603,7 @@ def test_captured_and_replayed(hip):
     """The three operators in one captured graph, replayed with other data, lengths and eager work in between; the workspace
     grows between the replays (the graph's stays)."""
     say("[batch] capture and replay")
-    heads, kv, hd, prefix, cap, tokens, dt = 8, 2, 64, 300, 40, 3, DType.BF16
+    heads, kv, hd, prefix, cap, tokens, dt = 8, 2, 64, 900, 40, 3, DType.BF16
     lens = [40, 11, 3]
     b, n, vocab = 3, 2, 9000
     be = HipBackend(0)   # its workspace starts empty

@@ -92,6 +92,11 @@ int main() {
             CHECK(p.ml_bytes + p.o_bytes == p.bytes());
         }
     }
+    // the shapes of the GPU tests take both ways
+    CHECK(prefix_plan(33, 20, 3, 1, 8, 2, 64, 2, 256).direct && prefix_plan(33, 20, 3, 1, 8, 2, 64, 4, 256).direct);
+    CHECK(!prefix_plan(300, 70, 4, 5, 6, 2, 80, 4, 256).direct && prefix_plan(300, 70, 4, 5, 6, 2, 80, 2, 256).direct);
+    CHECK(!prefix_plan(520, 600, 4, 1, 2, 2, 8, 2, 256).direct && !prefix_plan(1333, 90, 40, 1, 8, 2, 128, 2, 256).direct);
+    CHECK(!prefix_plan(600, 40, 3, 4, 4, 2, 64, 2, 256).direct && !prefix_plan(600, 40, 3, 4, 4, 2, 64, 4, 256).direct);
     printf("ok\n");
     return 0;
 }

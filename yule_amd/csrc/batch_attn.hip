@@ -473,35 +473,48 @@ struct WaveAttn<float, D> {
     }
 };
 
-// ---- a workgroup: NW waves share 32 slots and take the keys' subtiles in turn
-template <typename T, uint32_t D>
+// Keys k0 .. k1 - 1 of some rows: a slot sees those below lim (each lane's own), every
+// slot those below lim_all.
+struct Span {
+    Rows K, V;
+    uint32_t k0, k1, lim, lim_all;
+};
+
+// ---- a workgroup: NW waves share 32 slots and take the spans' subtiles in turn
+template <typename T, uint32_t D, uint32_t N>
 struct BlockAttn {
     using W = WaveAttn<T, D>;
     static constexpr uint32_t NW = 4;
     // waves a SIMD that the LDS has room for: the registers are to allow them too
-    static constexpr uint32_t WAVES = W::LDS <= 8192 ? 4 : W::LDS <= 12288 ? 3 : W::LDS <= 16384 ? 2 : 1;
+    static constexpr uint32_t WAVES = W::LDS <= 8192 ? (N > 1 ? 3 : 4) : W::LDS <= 12288 ? 3 : W::LDS <= 16384 ? 2 : 1;
     struct Shared {
         __align__(1024) uint8_t tiles[NW][W::LDS];
         float m[NW][32], l[NW][32];
-        uint32_t lim[32], dropped[NW];
+        uint32_t lim[N][32], dropped[NW];
     };
 
     // out(slot of 32, dim, four sums, maximum, weight): joined over the waves
     template <typename OUT>
-    __device__ __forceinline__ static void run(Shared &sh, const uint8_t *qrow, const Rows &K, const Rows &V,
-                                               uint32_t hb, uint32_t k0, uint32_t k1, uint32_t lim, uint32_t lim_all,
-                                               float c, OUT out) {
+    __device__ __forceinline__ static void run(Shared &sh, const uint8_t *qrow, const Span (&sp)[N], uint32_t hb, float c,
+                                               OUT out) {
         const uint32_t tid = threadIdx.x, lane = tid & 63u, h = lane >> 5, r32 = lane & 31u;
         const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         W w;
         w.init(qrow, hb, h);
-        lim_all = lim_all < k1 ? lim_all : k1;
-        const bool dropped = w.walk(K, V, hb, k0 + 32 * wave, 32 * NW, k1, lim, lim_all, sh.tiles[wave], lane, c);
+        bool dropped = false;
+        uint32_t turn = wave;   // the wave's first subtile of a span
+#pragma unroll
+        for (uint32_t n = 0; n < N; n++) {
+            const Span &x = sp[n];
+            dropped |= w.walk(x.K, x.V, hb, x.k0 + 32 * turn, 32 * NW, x.k1, x.lim, x.lim_all < x.k1 ? x.lim_all : x.k1,
+                              sh.tiles[wave], lane, c);
+            turn = (turn - (x.k1 - x.k0 + 31) / 32) % NW;
+            if (h == 0) sh.lim[n][r32] = x.lim;   // (the same from every wave)
+        }
         const float l = w.l + __shfl_xor(w.l, 32, 64);
         if (h == 0) {
             sh.m[wave][r32] = w.m;
             sh.l[wave][r32] = l;
-            sh.lim[r32] = lim;   // (the same from every wave)
         }
         if (lane == 0) sh.dropped[wave] = dropped;
         // the wave's subtiles make room for its sums, f32 [32][D], chunks XORed with the row (the writes of
@@ -533,8 +546,15 @@ struct BlockAttn {
                 acc += f * o;
             }
             // (dropped from the first subtile on that some slot does not see whole)
-            if (any && 16 * ch < 4 * hb / W::SZ)
-                acc = add_not_finite<T>(acc, V.p + 4 * ch * W::SZ, V.stride, lim_all < k0 ? k0 : lim_all - (lim_all - k0) % 32, sh.lim[r]);
+            if (any && 4 * ch * W::SZ < hb) {
+#pragma unroll
+                for (uint32_t n = 0; n < N; n++) {
+                    const Span &x = sp[n];
+                    const uint32_t whole = x.lim_all < x.k1 ? x.lim_all : x.k1;
+                    acc = add_not_finite<T>(acc, x.V.p + 4 * ch * W::SZ, x.V.stride, whole < x.k0 ? x.k0 : whole - (whole - x.k0) % 32,
+                                            sh.lim[n][r]);
+                }
+            }
             out(r, 4 * ch, acc, M, L);
         }
     }
@@ -812,9 +832,8 @@ __device__ __forceinline__ bool find_tile(const uint32_t *off, uint32_t n_seqs, 
 }
 
 template <typename T, uint32_t D>
-__global__ __launch_bounds__((64 * BlockAttn<T, D>::NW))
-    __attribute__((amdgpu_waves_per_eu(BlockAttn<T, D>::WAVES))) void prompt_attn_kernel(PromptArgs a) {
-    using B = BlockAttn<T, D>;
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(BlockAttn<T, D, 1>::WAVES))) void prompt_attn_kernel(PromptArgs a) {
+    using B = BlockAttn<T, D, 1>;
     __shared__ typename B::Shared sh;
     const uint32_t kvh = blockIdx.x % a.s.n_kv, lane = threadIdx.x & 63u;
     uint32_t row0, len, tile;
@@ -827,10 +846,10 @@ __global__ __launch_bounds__((64 * BlockAttn<T, D>::NW))
     };
     const uint32_t mine = slot0 + (lane & 31u) < last ? slot0 + (lane & 31u) : last;
     const Rows K = {a.k + (size_t)row0 * a.ks + (size_t)kvh * hb, a.ks}, V = {a.v + (size_t)row0 * a.vs + (size_t)kvh * hb, a.vs};
-    B::run(sh, a.q + at(mine, a.qs), K, V, hb, 0, last / a.s.group + 1u, mine / a.s.group + 1u, slot0 / a.s.group + 1u,
-           a.s.c, [&](uint32_t r, uint32_t d, f4v o, float, float L) {
-               if (slot0 + r <= last && d < a.s.hd) store4<T>(a.out + at(slot0 + r, a.os), d, o * (L == 0.f ? 0.f : 1.0f / L));
-           });
+    const Span seen[1] = {{K, V, 0, last / a.s.group + 1u, mine / a.s.group + 1u, slot0 / a.s.group + 1u}};
+    B::run(sh, a.q + at(mine, a.qs), seen, hb, a.s.c, [&](uint32_t r, uint32_t d, f4v o, float, float L) {
+        if (slot0 + r <= last && d < a.s.hd) store4<T>(a.out + at(slot0 + r, a.os), d, o * (L == 0.f ? 0.f : 1.0f / L));
+    });
 }
 
 // the same by workgroups of 128 slots
@@ -870,9 +889,9 @@ struct PrefixArgs {
 
 // TILE: the prefix by workgroups of 128 slots that share its tiles
 template <typename T, uint32_t D, bool TILE>
-__global__ __launch_bounds__((64 * BlockAttn<T, D>::NW))
-    __attribute__((amdgpu_waves_per_eu(TILE ? (D <= 128 ? 2 : 1) : BlockAttn<T, D>::WAVES))) void prefix_attn_kernel(PrefixArgs a) {
-    using B = BlockAttn<T, D>;
+__global__ __launch_bounds__(256)
+    __attribute__((amdgpu_waves_per_eu(TILE ? (D <= 128 ? 2 : 1) : BlockAttn<T, D, 1>::WAVES))) void prefix_attn_kernel(PrefixArgs a) {
+    using B = BlockAttn<T, D, 1>;
     using P = TileAttn<typename std::conditional<TILE, T, _Float16>::type, TILE ? D : 64, 1>;
     __shared__ union {
         typename B::Shared block;
@@ -906,7 +925,8 @@ __global__ __launch_bounds__((64 * BlockAttn<T, D>::NW))
                    });
         } else {
             const uint32_t slot0 = tile * kAttnTileRows, slot = slot0 + (lane & 31u);
-            B::run(sh.block, query(slot < slots ? slot : slots - 1u), K, V, hb, k0, k1, k1, k1, a.s.c,
+            const Span seen[1] = {{K, V, k0, k1, k1, k1}};
+            B::run(sh.block, query(slot < slots ? slot : slots - 1u), seen, hb, a.s.c,
                    [&](uint32_t i, uint32_t d, f4v o, float M, float L) {
                        if (slot0 + i >= slots || d >= a.s.hd) return;
                        const size_t at = part + pair(slot0 + i);
@@ -937,13 +957,42 @@ __global__ __launch_bounds__((64 * BlockAttn<T, D>::NW))
     }
     const Rows K = {a.kt + (size_t)seq * a.cap * a.kts + (size_t)kvh * hb, a.kts};
     const Rows V = {a.vt + (size_t)seq * a.cap * a.vts + (size_t)kvh * hb, a.vts};
-    B::run(sh.block, query(mine), K, V, hb, k0, k1, sees(mine) < k1 ? sees(mine) : k1, sees(slot0), a.s.c,
-           [&](uint32_t i, uint32_t d, f4v o, float M, float L) {
-               if (slot0 + i > last || d >= a.s.hd) return;
-               const size_t at = part + pair(slot0 + i);
-               if (d == 0) a.ml[at] = make_float2(M, L);
-               *reinterpret_cast<f4v *>(a.o + at * a.s.hd + d) = o;
-           });
+    const Span seen[1] = {{K, V, k0, k1, sees(mine) < k1 ? sees(mine) : k1, sees(slot0)}};
+    B::run(sh.block, query(mine), seen, hb, a.s.c, [&](uint32_t i, uint32_t d, f4v o, float M, float L) {
+        if (slot0 + i > last || d >= a.s.hd) return;
+        const size_t at = part + pair(slot0 + i);
+        if (d == 0) a.ml[at] = make_float2(M, L);
+        *reinterpret_cast<f4v *>(a.o + at * a.s.hd + d) = o;
+    });
+}
+
+// The same without chunks, in one launch: a workgroup walks the prefix and then its
+// sequence's tail.
+template <typename T, uint32_t D>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(BlockAttn<T, D, 2>::WAVES))) void prefix_short_kernel(
+    PrefixArgs a, uint8_t *out, uint32_t os) {
+    using B = BlockAttn<T, D, 2>;
+    __shared__ typename B::Shared sh;
+    const uint32_t lane = threadIdx.x & 63u, hb = a.s.hd * sizeof(T), g = a.s.group, kvh = blockIdx.x % a.s.n_kv;
+    const uint32_t job = blockIdx.x / a.s.n_kv, tile = job % a.t_tiles, seq = job / a.t_tiles;
+    const uint32_t len = a.lens[seq] < a.cap ? a.lens[seq] : a.cap, row0 = seq * a.n_tokens;
+    const uint32_t slots = a.n_tokens * g, slot0 = tile * kAttnTileRows;
+    const uint32_t last = slot0 + kAttnTileRows < slots ? slot0 + kAttnTileRows - 1u : slots - 1u;
+    const uint32_t mine = slot0 + (lane & 31u) < last ? slot0 + (lane & 31u) : last;
+    auto sees = [&](uint32_t slot) {
+        const uint32_t n = len + 1u + slot / g;
+        return n > a.n_tokens ? n - a.n_tokens : 0u;
+    };
+    auto at = [&](uint32_t slot, uint32_t stride) {
+        const uint32_t r = slot / g;
+        return (size_t)(row0 + r) * stride + (size_t)(kvh * g + (slot - r * g)) * hb;
+    };
+    const Span seen[2] = {{{a.kp + (size_t)kvh * hb, a.kps}, {a.vp + (size_t)kvh * hb, a.vps}, 0, a.prefix, a.prefix, a.prefix},
+                          {{a.kt + (size_t)seq * a.cap * a.kts + (size_t)kvh * hb, a.kts},
+                           {a.vt + (size_t)seq * a.cap * a.vts + (size_t)kvh * hb, a.vts}, 0, sees(last), sees(mine), sees(slot0)}};
+    B::run(sh, a.q + at(mine, a.qs), seen, hb, a.s.c, [&](uint32_t i, uint32_t d, f4v o, float, float L) {
+        if (slot0 + i <= last && d < a.s.hd) store4<T>(out + at(slot0 + i, os), d, o * (L == 0.f ? 0.f : 1.0f / L));
+    });
 }
 
 // out = sum_c 2^(m_c - M) o_c / sum_c 2^(m_c - M) l_c over a row's chunks, a
@@ -1072,6 +1121,14 @@ static int launch_prefix(hipStream_t s, const PrefixArgs &a, uint32_t dtype, uin
     return check_launch("prefix_attn");
 }
 
+static int launch_prefix_short(hipStream_t s, const PrefixArgs &a, uint8_t *out, uint32_t os, uint32_t dtype) {
+    const dim3 grid(a.s.n_kv * a.t_tiles * a.n_seqs);
+    by_shape(dtype, a.s.hd, [&](auto t, auto d) {
+        hipLaunchKernelGGL((prefix_short_kernel<decltype(t), decltype(d)::value>), grid, dim3(256), 0, s, a, out, os);
+    });
+    return check_launch("prefix_attn");
+}
+
 static int launch_join(hipStream_t s, const PrefixArgs &a, uint8_t *out, uint32_t os, uint32_t dtype) {
     const uint32_t n_heads = a.s.group * a.s.n_kv, rows = a.n_seqs * a.n_tokens * n_heads, hd = a.s.hd, parts = a.n_p + a.n_t;
     by_shape(dtype, hd, [&](auto t, auto d) {
@@ -1176,7 +1233,7 @@ int yule_hip_prefix_attn(yule_hip_backend *be, const yule_rows *q, const yule_ro
         if (p.rows > kMaxWorkgroups || p.p_jobs + p.t_jobs > kMaxWorkgroups)
             return set_error(YULE_ERR_INVALID, "prefix_attn: too many rows for one call");
         ScratchLease ws;   // held until both launches are enqueued
-        if ((rc = get_scratch(be, p.bytes(), &ws))) return rc;
+        if (!p.direct && (rc = get_scratch(be, p.bytes(), &ws))) return rc;
         PrefixArgs a = {};
         a.q = cq.p, a.kp = ckp.p, a.vp = cvp.p, a.kt = ckt.p, a.vt = cvt.p;
         a.qs = cq.stride, a.kps = ckp.stride, a.vps = cvp.stride, a.kts = ckt.stride, a.vts = cvt.stride;
@@ -1184,9 +1241,10 @@ int yule_hip_prefix_attn(yule_hip_backend *be, const yule_rows *q, const yule_ro
         a.prefix = prefix_len, a.cap = tail_cap, a.n_seqs = n_seqs, a.n_tokens = n_tokens;
         a.p_chunk = p.p_chunk, a.n_p = p.n_p, a.p_tiles = p.p_tiles;
         a.t_chunk = p.t_chunk, a.n_t = p.n_t, a.t_tiles = p.t_tiles, a.p_jobs = (uint32_t)(p.p_jobs / n_kv_heads);
+        a.s = head_shape(n_heads, n_kv_heads, head_dim);
+        if (p.direct) return launch_prefix_short(be->stream, a, co.p, co.stride, dtype);
         a.ml = static_cast<float2 *>(ws.ptr);
         a.o = reinterpret_cast<float *>(static_cast<uint8_t *>(ws.ptr) + p.ml_bytes);
-        a.s = head_shape(n_heads, n_kv_heads, head_dim);
         if (p.p_jobs + p.t_jobs && (rc = launch_prefix(be->stream, a, dtype, p.p_jobs + p.t_jobs, p.p_slots > kAttnTileRows))) return rc;
         return launch_join(be->stream, a, co.p, co.stride, dtype);
     });

@@ -96,7 +96,15 @@ constexpr uint32_t kMaxParts = 1024;
 // ---- prefix_attn: the prefix and each tail in chunks of keys, one workgroup
 // each; a chunk's results (unnormalised sums, maximum and weight of the softmax)
 // go to the workspace and are joined by a second launch.
+// Few keys: one launch, a workgroup walks the prefix and its sequence's tail.  16-bit
+// types up to 512 keys (MI355X, bf16, 32/8x128: 8 sequences of 5 tokens, 300 + 200
+// keys, 9.9 us against 13.4 by chunks; 700 + 300 keys 13.8 against 10.8).  f32,
+// whose products take eight times as long: where a sequence's pairs fill its tiles
+// (64 sequences of 8 tokens, 300 + 200 keys: 47 against 68 us), and otherwise
+// up to 128 keys, a subtile a wave, as the prefix shares its tiles between the
+// sequences (64 of 1 token, 300 + 200 keys: 79 against 48).
 struct PrefixPlan {
+    bool direct;
     uint32_t p_chunk, n_p;   // keys of a prefix chunk, chunks (0 without a prefix)
     uint32_t t_chunk, n_t;   // the same of a tail
     uint32_t p_slots;            // (query row, head of the group) pairs of a prefix tile
@@ -134,6 +142,7 @@ inline PrefixPlan prefix_plan(uint32_t prefix_len, uint32_t tail_cap, uint32_t n
     split(tail_cap, per_t, (prefix_len ? 1ull : 2ull) * cus, &p.t_chunk, &p.n_t);
     const uint64_t t_jobs = p.n_t * per_t;
     split(prefix_len, (uint64_t)p.p_tiles * n_kv, 2ull * cus - (t_jobs < cus ? t_jobs : cus), &p.p_chunk, &p.n_p);
+    p.direct = (uint64_t)prefix_len + tail_cap <= (elem == 2 || n_tokens * group >= kAttnTileRows ? 512u : 128u);
     p.rows = (uint64_t)n_seqs * n_tokens * n_heads;
     p.p_jobs = (uint64_t)p.n_p * p.p_tiles * n_kv;
     p.t_jobs = (uint64_t)p.n_t * p.t_tiles * n_kv * n_seqs;
