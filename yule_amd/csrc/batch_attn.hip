@@ -1000,7 +1000,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(BlockAttn<T
 // groups of G lanes (four dims each) take the chunks in turn, so that their
 // loads do not wait for each other.  A row that saw no key has l = 0 everywhere
 // and gives zeros.
-template <typename T, uint32_t NT, uint32_t G>
+template <typename T, uint32_t NT, uint32_t G, uint32_t AHEAD>
 __global__ __launch_bounds__(NT) void prefix_join_kernel(const float2 *__restrict__ ml, const float *__restrict__ o,
                                                          uint8_t *__restrict__ out, uint32_t os, uint32_t rows,
                                                          uint32_t n_heads, uint32_t hd, uint32_t parts) {
@@ -1009,6 +1009,12 @@ __global__ __launch_bounds__(NT) void prefix_join_kernel(const float2 *__restric
     __shared__ float red[2][NW];
     __shared__ f4v sums[NG][G];
     const uint32_t at = blockIdx.x, tid = threadIdx.x, lane = tid & 63u, g = tid / G, d = 4 * (tid % G);
+    // a group's first AHEAD sums are on their way while the factors are worked out
+    const float *mine = o + (size_t)at * hd + (d < hd ? d : 0u);
+    const size_t step = (size_t)rows * hd;
+    f4v first[AHEAD + 1];
+#pragma unroll
+    for (uint32_t i = 0; i < AHEAD; i++) first[i] = *reinterpret_cast<const f4v *>(mine + (g + i * NG < parts ? g + i * NG : 0u) * step);
     float M = -INFINITY;
     for (uint32_t p = tid; p < parts; p += NT) M = fmaxf(M, ml[(size_t)p * rows + at].x);
 #pragma unroll
@@ -1032,14 +1038,16 @@ __global__ __launch_bounds__(NT) void prefix_join_kernel(const float2 *__restric
     if (lane == 0) red[1][tid >> 6] = L;
     __syncthreads();
     f4v acc = {0.f, 0.f, 0.f, 0.f};
-    if (d < hd) {
-        const float *mine = o + (size_t)at * hd + d;
-        const size_t step = (size_t)rows * hd;
+#pragma unroll
+    for (uint32_t i = 0; i < AHEAD; i++) {
+        const uint32_t p = g + i * NG;
+        const float e = p < parts ? f[p] : -1.f;
+        if (e != -1.f) acc += e * first[i];
+    }
 #pragma unroll 4
-        for (uint32_t p = g; p < parts; p += NG) {
-            const float e = f[p];
-            if (e != -1.f) acc += e * *reinterpret_cast<const f4v *>(mine + p * step);
-        }
+    for (uint32_t p = g + AHEAD * NG; p < parts; p += NG) {
+        const float e = f[p];
+        if (e != -1.f) acc += e * *reinterpret_cast<const f4v *>(mine + p * step);
     }
     sums[g][tid % G] = acc;
     __syncthreads();
@@ -1134,11 +1142,20 @@ static int launch_join(hipStream_t s, const PrefixArgs &a, uint8_t *out, uint32_
     by_shape(dtype, hd, [&](auto t, auto d) {
         using T = decltype(t);
         constexpr uint32_t D = decltype(d)::value, G = D <= 64 ? 16 : D <= 128 ? 32 : 64;
-        // one wave where it takes every chunk in a step or two
-        if (parts <= 2 * 64 / G)
-            hipLaunchKernelGGL((prefix_join_kernel<T, 64, G>), dim3(rows), dim3(64), 0, s, a.ml, a.o, out, os, rows, n_heads, hd, parts);
-        else
-            hipLaunchKernelGGL((prefix_join_kernel<T, 256, G>), dim3(rows), dim3(256), 0, s, a.ml, a.o, out, os, rows, n_heads, hd, parts);
+        auto go = [&](auto nt, auto ahead) {
+            constexpr uint32_t NT = decltype(nt)::value;
+            hipLaunchKernelGGL((prefix_join_kernel<T, NT, G, decltype(ahead)::value>), dim3(rows), dim3(NT), 0, s, a.ml, a.o,
+                               out, os, rows, n_heads, hd, parts);
+        };
+        using N = std::integral_constant<uint32_t, 0>;
+        using One = std::integral_constant<uint32_t, 64>;
+        using Four = std::integral_constant<uint32_t, 256>;
+        // One wave where it takes every chunk in a step or two.  Loads ahead where a group has more than four chunks:
+        // 60 of them, 156 rows: 12.7 us of the two launches against 14.7; 12 or 32 chunks, with as many loads for
+        // nothing, 17.1 against 16.8 and 53.5 against 51.5.
+        if (parts <= 2 * 64 / G) go(One{}, N{});
+        else if (parts <= 4 * 256 / G) go(Four{}, N{});
+        else go(Four{}, std::integral_constant<uint32_t, 8>{});
     });
     return check_launch("prefix_attn (join)");
 }
