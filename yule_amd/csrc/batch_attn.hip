@@ -581,7 +581,7 @@ struct TileAttn {
     // Keys k0 .. k1 - 1 of the workgroup, every slot of which sees those below
     // lim_all; the wave's slots see keys below lim (each lane's own), all of them
     // those below lim_lo, none those from lim_hi (0: the wave has no slots).
-    // out(dim, four sums, maximum, weight) of the lane's slot.
+    // out(LDS of the wave, sums, maximum, weight).
     template <typename OUT>
     __device__ __forceinline__ static void run(Shared &sh, const uint8_t *qrow, const Rows &K, const Rows &V, uint32_t hb,
                                                uint32_t k0, uint32_t k1, uint32_t lim, uint32_t lim_all, uint32_t lim_lo,
@@ -752,17 +752,21 @@ struct TileAttn {
                     for (int e = 0; e < 4; e++) w.o[t][4 * a + e] = w.o[t][4 * a + e] * f0 + x[e] * f1;
                 }
         }
+        if (any) {   // (dropped from the first tile on that some slot of the workgroup does not see whole)
 #pragma unroll
-        for (uint32_t t = 0; t < W::DT; t++)
+            for (uint32_t t = 0; t < W::DT; t++)
 #pragma unroll
-            for (uint32_t a = 0; a < 4; a++) {
-                const uint32_t d = 32 * t + 8 * a + 4 * h;
-                f4v o = {w.o[t][4 * a], w.o[t][4 * a + 1], w.o[t][4 * a + 2], w.o[t][4 * a + 3]};
-                // (dropped from the first tile on that some slot of the workgroup does not see whole)
-                if (any && d * W::SZ < hb)
-                    o = add_not_finite<T>(o, V.p + d * W::SZ, V.stride, lim_all < k0 ? k0 : lim_all - (lim_all - k0) % KEYS, lim);
-                out(d, o, M, l);
-            }
+                for (uint32_t a = 0; a < 4; a++) {
+                    const uint32_t d = 32 * t + 8 * a + 4 * h;
+                    f4v o = {w.o[t][4 * a], w.o[t][4 * a + 1], w.o[t][4 * a + 2], w.o[t][4 * a + 3]};
+                    if (d * W::SZ < hb)
+                        o = add_not_finite<T>(o, V.p + d * W::SZ, V.stride, lim_all < k0 ? k0 : lim_all - (lim_all - k0) % KEYS, lim);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) w.o[t][4 * a + e] = o[e];
+                }
+        }
+        // (KS 2: where this wave has just read its partner's sums)
+        out(&sh.kv[0][0][0][0] + (KS > 1 ? 128 * D : sizeof(sh.kv) / NW) * wave, w.o, M, l);
     }
 };
 
@@ -774,6 +778,33 @@ __device__ __forceinline__ void store4(uint8_t *row, uint32_t d, f4v x) {
     } else {
         typedef T t4 __attribute__((ext_vector_type(4)));
         *reinterpret_cast<t4 *>(row + 2 * d) = t4{(T)x[0], (T)x[1], (T)x[2], (T)x[3]};
+    }
+}
+
+// The wave's slots' rows, whole lines at a time: o as the lanes hold it through the
+// wave's part of the LDS.  Straight from the registers a store would touch 32 rows
+// for 16 bytes each (20 prompts of 100 rows, bf16: 20.9 us, so 18.5).  row: this lane's slot's (lane and lane + 32 the same),
+// null if it has none; hb: bytes of the head.
+template <typename T, uint32_t D>
+__device__ __forceinline__ void store_rows(uint8_t *lds, const f16v (&o)[D / 32], float inv, uint8_t *row, uint32_t hb, uint32_t lane) {
+    constexpr uint32_t C = D * sizeof(T) / 16;
+    const uint32_t r32 = lane & 31u, h = lane >> 5;
+#pragma unroll
+    for (uint32_t t = 0; t < D / 32; t++)
+#pragma unroll
+        for (uint32_t a = 0; a < 4; a++) {
+            const uint32_t byte = (32 * t + 8 * a + 4 * h) * sizeof(T);
+            const f4v v = {o[t][4 * a], o[t][4 * a + 1], o[t][4 * a + 2], o[t][4 * a + 3]};
+            store4<T>(lds + r32 * (16 * C) + (((byte >> 4) ^ swizzle<C, 1>(r32)) << 4) + (byte & 15u), 0, v * inv);
+        }
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);   // (other lanes' values next; a wave's LDS accesses are in order)
+    const uint64_t at = reinterpret_cast<uint64_t>(row);
+#pragma unroll
+    for (uint32_t i = 0; i < 32 * C / 64; i++) {
+        const uint32_t L = 64 * i + lane, r = L / C, ch = L % C;
+        const i4v v = *reinterpret_cast<const i4v *>(lds + r * (16 * C) + ((ch ^ swizzle<C, 1>(r)) << 4));
+        const uint64_t to = (uint64_t)(uint32_t)__shfl((int)(at >> 32), (int)r, 64) << 32 | (uint32_t)__shfl((int)(uint32_t)at, (int)r, 64);
+        if (to && 16 * ch < hb) *reinterpret_cast<i4v *>(to + 16 * ch) = v;
     }
 }
 
@@ -868,10 +899,10 @@ __global__ __launch_bounds__(256 * KS) __attribute__((amdgpu_waves_per_eu(D <= 1
     const size_t head = (size_t)(kvh * g + (mine - r * g)) * hb;
     const Rows K = {a.k + (size_t)row0 * a.ks + (size_t)kvh * hb, a.ks}, V = {a.v + (size_t)row0 * a.vs + (size_t)kvh * hb, a.vs};
     const bool any = first_w <= last, own = first_w + (lane & 31u) <= last;
-    uint8_t *const out = a.out + (size_t)(row0 + r) * a.os + head;
+    uint8_t *const out = own ? a.out + (size_t)(row0 + r) * a.os + head : nullptr;
     B::run(sh, a.q + (size_t)(row0 + r) * a.qs + head, K, V, hb, 0, last / g + 1u, r + 1u, slot0 / g + 1u, any ? first_w / g + 1u : 0u,
-           any ? last_w / g + 1u : 0u, a.s.c, [&](uint32_t d, f4v o, float, float L) {
-               if (own && d < a.s.hd) store4<T>(out, d, o * (L == 0.f ? 0.f : 1.0f / L));
+           any ? last_w / g + 1u : 0u, a.s.c, [&](uint8_t *lds, f16v (&o)[D / 32], float, float L) {
+               store_rows<T, D>(lds, o, L == 0.f ? 0.f : 1.0f / L, out, hb, lane);
            });
 }
 
@@ -918,10 +949,17 @@ __global__ __launch_bounds__(256)
             const uint32_t mine = slot < slots ? slot : slots - 1u;
             const size_t at = part + pair(mine);
             P::run(sh.tile, query(mine), K, V, hb, k0, k1, k1, k1, first < slots ? k1 : 0u, first < slots ? k1 : 0u, a.s.c,
-                   [&](uint32_t d, f4v o, float M, float L) {
-                       if (slot >= slots || d >= a.s.hd) return;
-                       if (d == 0) a.ml[at] = make_float2(M, L);
-                       *reinterpret_cast<f4v *>(a.o + at * a.s.hd + d) = o;
+                   [&](uint8_t *, f16v (&o)[D / 32], float M, float L) {
+                       if (slot >= slots) return;
+                       if (lane < 32) a.ml[at] = make_float2(M, L);
+#pragma unroll
+                       for (uint32_t t = 0; t < D / 32; t++)
+#pragma unroll
+                           for (uint32_t x = 0; x < 4; x++) {
+                               const uint32_t d = 32 * t + 8 * x + 4 * (lane >> 5);
+                               if (d < a.s.hd)
+                                   *reinterpret_cast<f4v *>(a.o + at * a.s.hd + d) = f4v{o[t][4 * x], o[t][4 * x + 1], o[t][4 * x + 2], o[t][4 * x + 3]};
+                           }
                    });
         } else {
             const uint32_t slot0 = tile * kAttnTileRows, slot = slot0 + (lane & 31u);
