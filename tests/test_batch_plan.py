@@ -87,7 +87,7 @@ int main() {
         CHECK((uint64_t)p.t_tiles * kAttnTileRows >= (uint64_t)tokens * group);
         CHECK(p.p_jobs == (uint64_t)p.n_p * p.p_tiles * kv && p.t_jobs == (uint64_t)p.n_t * p.t_tiles * kv * seqs);
         if (p.n_p + p.n_t) {
-            const uint64_t last = p.ml_at(p.n_p + p.n_t - 1, p.rows - 1);
+            const uint64_t last = (uint64_t)(p.n_p + p.n_t - 1) * p.rows + p.rows - 1;   // the last chunk's last row
             CHECK((last + 1) * 8 <= p.ml_bytes && p.ml_bytes % 256 == 0 && (last + 1) * hd * 4 <= p.o_bytes);
             CHECK(p.ml_bytes + p.o_bytes == p.bytes());
         }

@@ -7,7 +7,7 @@
 // read serves every head of the group.  A wave holds 32 slots and walks its keys
 // in subtiles of 32 with an online softmax:
 //   S^T = K Q^T      keys x slots, a lane holds 16 keys of one slot
-//   p = 2^(c S - m), m the running maximum of c S, c = log2(e) / sqrt(hd)
+//   p = 2^(c S - m), m a running maximum of c S (up to kLag behind), c = log2(e) / sqrt(hd)
 //   O^T += V^T P^T   dims x slots; the lane's p are the operand as they lie
 // on the 32-row matrix instructions (operand row or column = lane % 32, k from h
 // = lane / 32; result column = lane % 32, row = 8 (i / 4) + 4 h + i % 4).  The
@@ -47,8 +47,9 @@ __device__ __forceinline__ f16v mma16(i4v a, i4v b, f16v c) {
     }
 }
 
-// eight probabilities as an operand, rounded to the type (2^-9 or 2^-12 of each
-// value at most: below the rounding of V itself; the weight's sum keeps f32)
+// Eight weights as an operand, rounded to the type: 2^-8 (bf16) or 2^-11 of each at
+// most, as much as the result's own rounding, and of either sign, so that the two
+// together stay below 1.5 times the one.  The weights' sum keeps f32.
 template <typename T>
 __device__ __forceinline__ i4v pack8(const f16v &s, int at) {
     if constexpr (__is_same(T, _Float16)) {
@@ -271,26 +272,23 @@ struct WaveAttn {
     }
     template <typename F>
     __device__ __forceinline__ void values(const f16v &s, const uint8_t *v, uint32_t lane, F also) {
-        const uint32_t h = lane >> 5;
-        {
-            // the transposing read gives lane l of 16 column l of the four rows that lanes 4 r .. 4 r + 3 point
-            // to: here the dims of V^T's rows from four keys
-            const uint32_t e = lane & 15u, g = lane >> 4;
+        // the transposing read gives lane l of 16 column l of the four rows that lanes 4 r .. 4 r + 3 point to: here the
+        // dims of V^T's rows from four keys
+        const uint32_t h = lane >> 5, e = lane & 15u, g = lane >> 4;
 #pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const i4v p = pack8<T>(s, 8 * k);
-                const uint32_t r0 = 16 * k + 4 * h + (e >> 2), r1 = r0 + 8;
+        for (int k = 0; k < 2; k++) {
+            const i4v p = pack8<T>(s, 8 * k);
+            const uint32_t r0 = 16 * k + 4 * h + (e >> 2), r1 = r0 + 8;
 #pragma unroll
-                for (uint32_t t = 0; t < DT; t++) {
-                    const uint32_t ch = 4 * t + 2 * (g & 1u) + ((e & 3u) >> 1), sub = 8 * (e & 1u);
-                    const s4v a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (lds_s4)(lds_b)(v + r0 * RB + ((ch ^ swizzle<C, 2>(r0)) << 4) + sub));
-                    const s4v a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (lds_s4)(lds_b)(v + r1 * RB + ((ch ^ swizzle<C, 2>(r1)) << 4) + sub));
-                    const auto a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
-                    o[t] = mma16<T>(__builtin_bit_cast(i4v, a), p, o[t]);
-                    also(DT * k + t);
-                }
+            for (uint32_t t = 0; t < DT; t++) {
+                const uint32_t ch = 4 * t + 2 * (g & 1u) + ((e & 3u) >> 1), sub = 8 * (e & 1u);
+                const s4v a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (lds_s4)(lds_b)(v + r0 * RB + ((ch ^ swizzle<C, 2>(r0)) << 4) + sub));
+                const s4v a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (lds_s4)(lds_b)(v + r1 * RB + ((ch ^ swizzle<C, 2>(r1)) << 4) + sub));
+                const auto a = __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7);
+                o[t] = mma16<T>(__builtin_bit_cast(i4v, a), p, o[t]);
+                also(DT * k + t);
             }
         }
     }
@@ -783,8 +781,9 @@ __device__ __forceinline__ void store4(uint8_t *row, uint32_t d, f4v x) {
 
 // The wave's slots' rows, whole lines at a time: o as the lanes hold it through the
 // wave's part of the LDS.  Straight from the registers a store would touch 32 rows
-// for 16 bytes each (20 prompts of 100 rows, bf16: 20.9 us, so 18.5).  row: this lane's slot's (lane and lane + 32 the same),
-// null if it has none; hb: bytes of the head.
+// for 16 bytes each (20 prompts of 100 rows, bf16: 20.9 us, so 18.5).  row: this
+// lane's slot's (lane and lane + 32 the same), null if it has none; hb: bytes of
+// the head.
 template <typename T, uint32_t D>
 __device__ __forceinline__ void store_rows(uint8_t *lds, const f16v (&o)[D / 32], float inv, uint8_t *row, uint32_t hb, uint32_t lane) {
     constexpr uint32_t C = D * sizeof(T) / 16;

@@ -26,8 +26,8 @@ inline uint32_t attn_padded_dim(uint32_t hd, uint32_t elem) {
 
 // Rows r < n_rows, each `width` elements of `elem` bytes, of a buffer of
 // buf_bytes: nullptr, or what is wrong.  align: bytes that every row starts at
-// a multiple of.  Row offsets inside 32 rows have to fit 31 bits (the copies
-// into LDS take 32-bit offsets from a 64-bit row address).
+// a multiple of.  Offsets inside a tile (32 rows of f32, 64 of 16-bit types) have
+// to fit 31 bits: the copies into LDS take 32-bit offsets from a 64-bit row address.
 inline const char *check_rows(uint64_t offset, uint64_t stride, uint64_t n_rows, uint64_t width, uint32_t elem,
                               uint64_t buf_bytes, uint32_t align) {
     if (!n_rows || !width) return nullptr;
@@ -64,8 +64,9 @@ constexpr uint32_t kMaxKeys = 1u << 30;   // of a prefix, and of a tail
 //          against 15.6 and 17.4)
 //   split  128 a workgroup of eight waves, half of which take every other tile of
 //          keys: few workgroups with a long way (32/8x128: 1000 rows 21.8 against
-//          23.3, 2000 rows 47.1 against 45.8; 12/2x80, 3000 rows: 40.8 against
-//          51.5; seven sequences of 259 rows on average 28.1 against 22.9)
+//          23.3, but 2000 rows, twice the workgroups, 47.1 against 45.8; 12/2x80,
+//          3000 rows: 40.8 against 51.5; but seven sequences of 259 rows on
+//          average 28.1 against 22.9)
 //   128    four waves of 32 over shared tiles of keys: throughput
 struct PromptPlan {
     uint32_t slots, split;   // pairs of a tile, groups of waves that share its keys
@@ -114,8 +115,6 @@ struct PrefixPlan {
     size_t ml_bytes, o_bytes;   // workspace: (m, l) pairs, then the sums
 
     size_t bytes() const { return ml_bytes + o_bytes; }
-    // indexes of a chunk's (m, l) pair and of its sums
-    uint64_t ml_at(uint32_t chunk, uint64_t row) const { return chunk * rows + row; }
 };
 
 inline PrefixPlan prefix_plan(uint32_t prefix_len, uint32_t tail_cap, uint32_t n_seqs, uint32_t n_tokens,
