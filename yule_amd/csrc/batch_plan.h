@@ -88,7 +88,8 @@ inline PromptPlan prompt_plan(uint32_t n_seqs, uint32_t n_rows, uint32_t n_heads
 // ---- verify_drafts: values of a row that a workgroup takes
 constexpr uint32_t kVerifyChunk = 4096, kMaxVocab = 1u << 30, kMaxDrafts = 1024;
 // sequences of one launch, and words between their tickets: a line of 128 bytes
-// each (512 workgroups that draw from one line queue for it: 15 us instead of 9)
+// each (512 workgroups that draw from one line queue for it: 16 rows of 128256
+// values 15.1 us, with a line each 10.7)
 constexpr uint32_t kVerifyTickets = 1024, kVerifyTicketWords = 32;
 
 // chunks of a prefix and a tail together
