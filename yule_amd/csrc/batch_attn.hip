@@ -143,7 +143,7 @@ __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)"
 // there, and not kept in registers over the loop (operand and copy addresses: a
 // few integer operations each, beside hundreds of registers)
 __device__ __forceinline__ uint32_t opaque(uint32_t x) {
-    asm volatile("" : "+v"(x));
+    asm volatile("; used" : "+v"(x));
     return x;
 }
 
@@ -242,7 +242,7 @@ struct WaveAttn {
     // every copy that is in flight then.
     __device__ __forceinline__ void wait_queries() {
 #pragma unroll
-        for (uint32_t s = 0; s < NS; s++) asm volatile("" : "+v"(q[s]));
+        for (uint32_t s = 0; s < NS; s++) asm volatile("; used" : "+v"(q[s]));
     }
     // S^T = K Q^T with K's subtile at k; also(i) after product i
     template <typename F>
@@ -433,7 +433,7 @@ struct WaveAttn<float, D> {
             for (uint32_t j = 0; j < DT; j++) copy(key, j);
         }
 #pragma unroll
-        for (uint32_t s = 0; s < NS; s++) asm volatile("" : "+v"(q[s]));   // (as wait_queries)
+        for (uint32_t s = 0; s < NS; s++) asm volatile("; used" : "+v"(q[s]));   // (as wait_queries)
         bool dropped = false;
         auto subtile = [&](auto masked) {
             const bool more = key + step < k1;
