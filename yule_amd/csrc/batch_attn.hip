@@ -387,7 +387,7 @@ struct WaveAttn<float, D> {
                                          uint32_t k1, uint32_t lim, uint32_t lim_all, uint8_t *lds, uint32_t lane,
                                          float c) {
         const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)reinterpret_cast<uintptr_t>((lds_b)lds));
-        if (hb < D * 4) {   // dims past the head stay zero: copies leave them out
+        if (hb < D * 4) {   // what the copies leave out starts as zeros
 #pragma unroll
             for (uint32_t i = 0; i < LDS / 1024; i++) *reinterpret_cast<i4v *>(lds + 1024 * i + 16 * lane) = i4v{0, 0, 0, 0};
             wait_lds();
@@ -443,9 +443,11 @@ struct WaveAttn<float, D> {
 #pragma unroll
             for (uint32_t j = 0; j < DT; j++) {   // S^T += K Q^T
                 wait_copies<4 * (DT - 1)>();
+                // (products past the head are left out: a row of V may still lie there, and 0 times an infinity is not 0)
+                const uint32_t n = j + 1 < DT ? 4u : (hb - 128 * j) / 32;
 #pragma unroll
                 for (uint32_t st = 0; st < 4; st++)
-                    s[0] = mma16<float>(*reinterpret_cast<const i4v *>(lds + ka[st] + PIECE * j), q[4 * j + st], s[0]);
+                    if (st < n) s[0] = mma16<float>(*reinterpret_cast<const i4v *>(lds + ka[st] + PIECE * j), q[4 * j + st], s[0]);
                 wait_lds();
                 copy(key, DT + j);
             }
