@@ -89,6 +89,24 @@ int yule_hip_copy_buffer_offset(yule_hip_backend *be, yule_buffer src, yule_buff
                                 size_t src_offset, size_t dst_offset, size_t size);
 int yule_hip_synchronize(yule_hip_backend *be);
 
+/* A handle over device memory that the caller owns, such as another library's
+ * tensor (no counterpart in the trait): calls read and write it where it lies.
+ * size bytes from ptr, a multiple of 16, inside one allocation on the backend's
+ * device; none of them may have a handle already, so that different handles are
+ * different memory (a slice is given by offset and stride where a call takes
+ * them).  The copies and the batched operators use the whole of it; the kernels
+ * of the other calls may read up to 64 bytes past their data, so for these the
+ * last 64 bytes count as behind the end.  The memory has to stay until the
+ * handle is freed: yule_hip_free waits for the backend's work and drops the
+ * handle, the memory stays the caller's.  Work on it elsewhere is ordered by
+ * the caller, through the backend's stream. */
+int yule_hip_import_buffer(yule_hip_backend *be, void *ptr, size_t size_bytes, yule_buffer *out);
+
+/* The backend's stream, a hipStream_t of the HIP runtime that the library is
+ * linked to, on which every call enqueues its work: what shares memory with the
+ * backend runs on it too, or waits by events.  It ends with the backend. */
+int yule_hip_stream(yule_hip_backend *be, void **out);
+
 /* ComputeBackend::matmul (lib.rs:26-34): C[m,n] = A[m,k] * B[k,n], f32 row-major */
 int yule_hip_matmul(yule_hip_backend *be, yule_buffer a, yule_buffer b, yule_buffer out,
                     uint32_t m, uint32_t n, uint32_t k);

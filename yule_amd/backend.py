@@ -36,6 +36,8 @@ _SIGS: dict[str, tuple] = {
     "yule_hip_copy_buffer": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint64, C.c_size_t]),
     "yule_hip_copy_buffer_offset": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint64, C.c_size_t, C.c_size_t, C.c_size_t]),
     "yule_hip_synchronize": (C.c_int, [C.c_void_p]),
+    "yule_hip_import_buffer": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.POINTER(C.c_uint64)]),
+    "yule_hip_stream": (C.c_int, [C.c_void_p, C.POINTER(C.c_void_p)]),
     "yule_hip_matmul": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint64, C.c_uint32, C.c_uint32, C.c_uint32]),
     "yule_hip_softmax": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint32]),
     "yule_hip_rms_norm": (C.c_int, [C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint64, C.c_uint32, C.c_float]),
@@ -252,6 +254,22 @@ class HipBackend:
 
     def synchronize(self) -> None:
         self._check(self._lib.yule_hip_synchronize(self._be))
+
+    def import_buffer(self, address: int, size_bytes: int) -> BufferHandle:
+        """A handle over device memory that the caller owns and keeps until the handle is
+        freed, such as a tensor of torch's at its data_ptr().  torch is imported before the
+        library is loaded, as the two have to share one HIP runtime."""
+        h = C.c_uint64()
+        self._check(self._lib.yule_hip_import_buffer(self._be, address, size_bytes, C.byref(h)))
+        return BufferHandle(h.value)
+
+    @property
+    def stream(self) -> int:
+        """The backend's stream, for torch.cuda.ExternalStream: work on imported memory belongs
+        on it, or waits for it."""
+        s = C.c_void_p()
+        self._check(self._lib.yule_hip_stream(self._be, C.byref(s)))
+        return s.value
 
     def matmul(self, a, b, out, m: int, n: int, k: int) -> None:
         self._check(self._lib.yule_hip_matmul(self._be, _h(a), _h(b), _h(out), m, n, k))

@@ -1240,7 +1240,7 @@ int yule_hip_prompt_attn(yule_hip_backend *be, const yule_rows *q, const yule_ro
             (rc = rows_arg(be, k, n_rows, kvd, elem, "prompt_attn (k)", &ck)) ||
             (rc = rows_arg(be, v, n_rows, kvd, elem, "prompt_attn (v)", &cv)) ||
             (rc = rows_arg(be, out, n_rows, qd, elem, "prompt_attn (out)", &co)) ||
-            (rc = get_buffer(be, offsets, ((size_t)n_seqs + 1) * 4, &off, "prompt_attn (offsets)")))
+            (rc = get_buffer(be, offsets, ((size_t)n_seqs + 1) * 4, &off, "prompt_attn (offsets)", 0, true)))
             return rc;
         if (out->buffer == q->buffer || out->buffer == k->buffer || out->buffer == v->buffer || out->buffer == offsets)
             return set_error(YULE_ERR_INVALID, "prompt_attn: an input and the output alias");
@@ -1277,7 +1277,7 @@ int yule_hip_prefix_attn(yule_hip_backend *be, const yule_rows *q, const yule_ro
             (tail_cap && ((rc = rows_arg(be, k_tail, tails, kvd, elem, "prefix_attn (k_tail)", &ckt)) ||
                           (rc = rows_arg(be, v_tail, tails, kvd, elem, "prefix_attn (v_tail)", &cvt)))) ||
             (rc = rows_arg(be, out, rows, qd, elem, "prefix_attn (out)", &co)) ||
-            (rc = get_buffer(be, tail_lens, (size_t)n_seqs * 4, &lens, "prefix_attn (tail_lens)")))
+            (rc = get_buffer(be, tail_lens, (size_t)n_seqs * 4, &lens, "prefix_attn (tail_lens)", 0, true)))
             return rc;
         if (out->buffer == q->buffer || out->buffer == tail_lens ||
             (prefix_len && (out->buffer == k_prefix->buffer || out->buffer == v_prefix->buffer)) ||

@@ -23,6 +23,7 @@ constexpr size_t kAllocSlack = 64;
 struct Buffer {
     void *ptr = nullptr;
     size_t size = 0;  // bytes requested by the caller (validation bound)
+    bool imported = false;  // the caller's memory: no slack behind it, and not freed
 };
 
 }  // namespace yule
@@ -60,9 +61,11 @@ namespace yule {
 int set_error(int code, const std::string &msg);
 int hip_error(hipError_t e, const char *what);
 
-// Look up a handle and check that [offset, offset+need) lies inside it.
+// Look up a handle and check that [offset, offset+need) lies inside it.  Of an
+// imported buffer the last kAllocSlack bytes count as behind its end, unless
+// the caller reads and writes nothing past `need` (exact).
 int get_buffer(yule_hip_backend *be, uint64_t h, size_t need, void **ptr, const char *what,
-               size_t offset = 0);
+               size_t offset = 0, bool exact = false);
 
 // Rows r < n_rows of an argument of a batched operator, `width` elements of
 // `elem` bytes each: address of the first (align: what every row starts at a

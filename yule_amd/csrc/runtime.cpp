@@ -76,16 +76,19 @@ int get_scratch(yule_hip_backend *be, size_t need, ScratchLease *lease) {
     return YULE_OK;
 }
 
-int get_buffer(yule_hip_backend *be, uint64_t h, size_t need, void **ptr, const char *what, size_t offset) {
+int get_buffer(yule_hip_backend *be, uint64_t h, size_t need, void **ptr, const char *what, size_t offset, bool exact) {
     std::lock_guard<std::mutex> lk(be->mu);
     auto it = be->buffers.find(h);
     if (it == be->buffers.end())
         return set_error(YULE_ERR_INVALID, std::string(what) + ": buffer " + std::to_string(h) + " not found");
-    if (offset > it->second.size || need > it->second.size - offset)
+    const Buffer &b = it->second;
+    const size_t size = !b.imported || exact ? b.size : b.size > kAllocSlack ? b.size - kAllocSlack : 0;
+    if (offset > size || need > size - offset)
         return set_error(YULE_ERR_INVALID, std::string(what) + ": access of " + std::to_string(need) +
                                                " bytes at offset " + std::to_string(offset) +
                                                " exceeds buffer " + std::to_string(h) + " of " +
-                                               std::to_string(it->second.size) + " bytes");
+                                               std::to_string(size) + " bytes" +
+                                               (size < b.size ? " (imported, less 64 of slack)" : ""));
     *ptr = static_cast<uint8_t *>(it->second.ptr) + offset;
     return YULE_OK;
 }
@@ -185,7 +188,8 @@ int yule_hip_destroy(yule_hip_backend *be) {
     if (!be) return YULE_OK;
     hipSetDevice(be->device);
     hipStreamSynchronize(be->stream);
-    for (auto &kv : be->buffers) hipFree(kv.second.ptr);
+    for (auto &kv : be->buffers)
+        if (!kv.second.imported) hipFree(kv.second.ptr);
     be->buffers.clear();
     if (be->scratch) hipFree(be->scratch);
     for (void *p : be->scratch_kept) hipFree(p);
@@ -241,25 +245,64 @@ int yule_hip_allocate(yule_hip_backend *be, size_t size, yule_buffer *out) {
 
 int yule_hip_free(yule_hip_backend *be, yule_buffer h) {
     YULE_CHECK_BE(be);
-    void *p = nullptr;
+    Buffer b;
     {
         std::lock_guard<std::mutex> lk(be->mu);
         auto it = be->buffers.find(h);
         if (it == be->buffers.end()) return YULE_OK;  // CpuBackend::free ignores unknown handles
-        p = it->second.ptr;
+        b = it->second;
         be->buffers.erase(it);
     }
     // queued kernels may still read the buffer
     int rc = hip_error(hipStreamSynchronize(be->stream), "free: synchronize");
-    hipFree(p);
+    if (!b.imported) hipFree(b.ptr);
     return rc;
+}
+
+int yule_hip_import_buffer(yule_hip_backend *be, void *ptr, size_t size, yule_buffer *out) {
+    return guarded("import_buffer", be, [&]() -> int {
+        if (!out) return set_error(YULE_ERR_INVALID, "import_buffer: null out");
+        if (!ptr || !size) return set_error(YULE_ERR_INVALID, "import_buffer: no memory");
+        if (reinterpret_cast<uintptr_t>(ptr) % 16) return set_error(YULE_ERR_INVALID, "import_buffer: not at a multiple of 16 bytes");
+        hipPointerAttribute_t at = {};
+        if (hipPointerGetAttributes(&at, ptr) != hipSuccess || at.type != hipMemoryTypeDevice) {
+            (void)hipGetLastError();
+            return set_error(YULE_ERR_INVALID, "import_buffer: not device memory of this process' HIP runtime");
+        }
+        if (at.device != be->device) return set_error(YULE_ERR_INVALID, "import_buffer: memory of another device");
+        hipDeviceptr_t base = nullptr;
+        size_t whole = 0;
+        int rc = hip_error(hipMemGetAddressRange(&base, &whole, ptr), "import_buffer: address range");
+        if (rc) return rc;
+        const size_t before = (size_t)(static_cast<uint8_t *>(ptr) - static_cast<uint8_t *>(base));
+        if (before > whole || size > whole - before) return set_error(YULE_ERR_INVALID, "import_buffer: reaches past the allocation");
+        const uint8_t *p0 = static_cast<uint8_t *>(ptr), *p1 = p0 + size;
+        std::lock_guard<std::mutex> lk(be->mu);
+        // calls tell their outputs from their inputs by the handle
+        for (const auto &kv : be->buffers) {
+            const uint8_t *q0 = static_cast<uint8_t *>(kv.second.ptr), *q1 = q0 + kv.second.size;
+            if (p0 < q1 && q0 < p1)
+                return set_error(YULE_ERR_INVALID, "import_buffer: overlaps buffer " + std::to_string(kv.first));
+        }
+        const uint64_t h = g_next_handle.fetch_add(1);
+        be->buffers[h] = Buffer{ptr, size, true};
+        *out = h;
+        return YULE_OK;
+    });
+}
+
+int yule_hip_stream(yule_hip_backend *be, void **out) {
+    YULE_CHECK_BE(be);
+    if (!out) return set_error(YULE_ERR_INVALID, "stream: null out");
+    *out = be->stream;
+    return YULE_OK;
 }
 
 int yule_hip_copy_to_device(yule_hip_backend *be, const void *data, size_t size, yule_buffer h) {
     YULE_CHECK_BE(be);
     if (!data && size) return set_error(YULE_ERR_INVALID, "copy_to_device: null data");
     void *p;
-    int rc = get_buffer(be, h, size, &p, "copy_to_device");
+    int rc = get_buffer(be, h, size, &p, "copy_to_device", 0, true);
     if (rc || !size) return rc;
     if ((rc = hip_error(hipMemcpyAsync(p, data, size, hipMemcpyHostToDevice, be->stream), "copy_to_device")))
         return rc;
@@ -270,7 +313,7 @@ int yule_hip_copy_from_device(yule_hip_backend *be, yule_buffer h, void *data, s
     YULE_CHECK_BE(be);
     if (!data && size) return set_error(YULE_ERR_INVALID, "copy_from_device: null data");
     void *p;
-    int rc = get_buffer(be, h, size, &p, "copy_from_device");
+    int rc = get_buffer(be, h, size, &p, "copy_from_device", 0, true);
     if (rc || !size) return rc;
     if ((rc = hip_error(hipMemcpyAsync(data, p, size, hipMemcpyDeviceToHost, be->stream), "copy_from_device")))
         return rc;
@@ -302,8 +345,8 @@ int yule_hip_copy_buffer_offset(yule_hip_backend *be, yule_buffer src, yule_buff
     YULE_CHECK_BE(be);
     void *ps, *pd;
     int rc;
-    if ((rc = get_buffer(be, src, size, &ps, "copy_buffer_offset (src)", src_offset))) return rc;
-    if ((rc = get_buffer(be, dst, size, &pd, "copy_buffer_offset (dst)", dst_offset))) return rc;
+    if ((rc = get_buffer(be, src, size, &ps, "copy_buffer_offset (src)", src_offset, true))) return rc;
+    if ((rc = get_buffer(be, dst, size, &pd, "copy_buffer_offset (dst)", dst_offset, true))) return rc;
     if (!size) return YULE_OK;
     return hip_error(hipMemcpyAsync(pd, ps, size, hipMemcpyDeviceToDevice, be->stream), "copy_buffer_offset");
 }

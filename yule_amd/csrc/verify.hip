@@ -262,11 +262,11 @@ extern "C" int yule_hip_verify_drafts(yule_hip_backend *be, const yule_rows *tar
         int rc;
         if ((rc = rows_ptr(be, target, rows_p, vocab, 4, 4, "verify_drafts (target)", &pp)) ||
             (n_draft && (rc = rows_ptr(be, draft, rows_q, vocab, 4, 4, "verify_drafts (draft)", &pq))) ||
-            (n_draft && (rc = get_buffer(be, draft_tokens, rows_q * 4, &pd, "verify_drafts (draft_tokens)"))) ||
-            (rc = get_buffer(be, uniforms, rows_p * 4, &pu, "verify_drafts (uniforms)")) ||
-            (draft_lens && (rc = get_buffer(be, draft_lens, (size_t)n_seqs * 4, &pl, "verify_drafts (draft_lens)"))) ||
-            (rc = get_buffer(be, accepted, (size_t)n_seqs * 4, &pa, "verify_drafts (accepted)")) ||
-            (rc = get_buffer(be, tokens, rows_p * 4, &pt, "verify_drafts (tokens)")))
+            (n_draft && (rc = get_buffer(be, draft_tokens, rows_q * 4, &pd, "verify_drafts (draft_tokens)", 0, true))) ||
+            (rc = get_buffer(be, uniforms, rows_p * 4, &pu, "verify_drafts (uniforms)", 0, true)) ||
+            (draft_lens && (rc = get_buffer(be, draft_lens, (size_t)n_seqs * 4, &pl, "verify_drafts (draft_lens)", 0, true))) ||
+            (rc = get_buffer(be, accepted, (size_t)n_seqs * 4, &pa, "verify_drafts (accepted)", 0, true)) ||
+            (rc = get_buffer(be, tokens, rows_p * 4, &pt, "verify_drafts (tokens)", 0, true)))
             return rc;
         const yule_buffer in[] = {target->buffer, n_draft ? draft->buffer : 0, n_draft ? draft_tokens : 0, uniforms, draft_lens};
         for (yule_buffer b : in)
