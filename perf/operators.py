@@ -157,39 +157,18 @@ def _hip():
     return _backend
 
 
-class Results(dict):
-    """Output buffers by name.  The backend's buffers are opaque handles and a program leaves its results on the
-    device between calls: a value is copied out when it is looked at."""
+class Handles:
+    """The backend's handles over a case's tensors, by name: the tensors are read and written where they lie."""
 
-    def __init__(self, holder, outputs):
-        super().__init__(outputs)
-        self.holder = holder
-
-    def __getitem__(self, name):
-        shape, dtype = super().__getitem__(name)
-        whole = dtype == torch.int64   # 32-bit ids on the device
-        host = np.empty(shape, np.uint32 if whole else np.float32 if dtype == torch.float32 else np.uint16)
-        self.holder.hip.copy_from_device(self.holder.h[name], host)
-        if whole:
-            return torch.from_numpy(host.astype(np.int64))
-        t = torch.from_numpy(host)
-        return t if dtype == torch.float32 else t.view(dtype)
-
-
-class Buffers:
-    """A case's tensors in the backend's buffers, by name."""
-
-    def __init__(self, tensors):
-        self.hip = _hip()
-        self.h = {}
-        for name, t in tensors.items():
-            if t.dtype in (torch.float16, torch.bfloat16):
-                t = t.view(torch.int16)
-            self.h[name] = self.hip.upload(t.cpu().numpy()) if t.numel() else self.hip.allocate(4)
+    def __init__(self, hip, tensors):
+        self.hip, self.tensors = hip, tensors
+        self.h = {name: hip.import_buffer(t.data_ptr(), t.numel() * t.element_size()) if t.numel() else None
+                  for name, t in tensors.items()}
 
     def __del__(self):
         for h in getattr(self, "h", {}).values():
-            self.hip.free(h)
+            if h is not None:
+                self.hip.free(h)
 
 
 class State:
@@ -203,31 +182,36 @@ def prepare(case, seed):
     if own:
         from yule_amd import DType
         from yule_amd.backend import Rows
-        kind = case["kind"]
+        hip, kind, n_seqs = _hip(), case["kind"], case.get("seqs")
+        # the program's stream is the backend's: torch's work and the operators' follow each other on it
+        stream = torch.cuda.ExternalStream(hip.stream)
+        stream.wait_stream(torch.cuda.current_stream())
+        torch.cuda.set_stream(stream)
         if kind == "verify":
-            outputs = {"accepted": ((case["seqs"],), torch.int64), "tokens": ((case["seqs"], case["drafts"] + 1), torch.int64)}
-            st.t.update({k: torch.zeros(s, dtype=torch.int32, device=_DEV) for k, (s, _) in outputs.items()})
+            # the ids that the operator writes, 32 bits each, and the program's 64-bit tokens
+            at, shape = -(-n_seqs // 4) * 4, (n_seqs, case["drafts"] + 1)
+            ids = torch.zeros(at + shape[0] * shape[1], dtype=torch.int32, device=_DEV)
+            st.t["accepted"], st.t["tokens"] = ids[:n_seqs], ids[at:]
+            st.ids, st.wide = ids.view(torch.uint32), torch.zeros(ids.shape, dtype=torch.int64, device=_DEV)
+            st.result = {"accepted": st.wide[:n_seqs], "tokens": st.wide[at:].view(shape)}
         else:
-            hd, dt = case["head_dim"], _TYPES[case["dtype"]]
-            qd, kvd = case["heads"] * hd, case["kv_heads"] * hd
             if kind == "prefix":
                 st.t["out"] = torch.zeros_like(st.t["q"])
             else:
                 st.n_seqs, st.n_rows = st.t["offsets"].numel() - 1, st.t["out"].shape[0]
-            outputs = {"out": (tuple(st.t["out"].shape), dt)}
+            st.result = {"out": st.t["out"]}
             st.dtype = DType[case["dtype"]]
-        st.b = Buffers(st.t)
-        st.t = None   # the data is in the backend's buffers now
-        st.result = Results(st.b, outputs)
+        st.b = Handles(hip, st.t)
         h = st.b.h
         if kind == "verify":
-            st.rows = {"p": Rows(h["p"], case["vocab"]), "q": Rows(h["q"], case["vocab"])}
-        elif kind == "prompt" and case["fused"]:
-            ld = qd + 2 * kvd
-            st.rows = {"q": Rows(h["qkv"], ld), "k": Rows(h["qkv"], ld, qd), "v": Rows(h["qkv"], ld, qd + kvd)}
+            st.rows = {n: Rows(h[n], case["vocab"]) if h[n] is not None else None for n in ("p", "q")}
         else:
-            st.rows = {n: Rows(h[n], qd if n == "q" else kvd) for n in h if n.split("_")[0] in ("q", "k", "v")}
-        if kind != "verify":
+            qd, kvd = case["heads"] * case["head_dim"], case["kv_heads"] * case["head_dim"]
+            if kind == "prompt" and case["fused"]:
+                ld = qd + 2 * kvd
+                st.rows = {"q": Rows(h["qkv"], ld), "k": Rows(h["qkv"], ld, qd), "v": Rows(h["qkv"], ld, qd + kvd)}
+            else:
+                st.rows = {n: Rows(h[n], qd if n == "q" else kvd) for n in h if n.split("_")[0] in ("q", "k", "v")}
             st.rows["out"] = Rows(h["out"], qd)
     return st
 
@@ -244,6 +228,7 @@ def _run_own(st):
     else:
         hip.verify_drafts(rows["p"], rows["q"], h["drafts"], h["uniforms"], h["lens"], h["accepted"], h["tokens"],
                           case["seqs"], case["drafts"], case["vocab"])
+        st.wide.copy_(st.ids)
     return st.result
 
 
