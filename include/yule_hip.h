@@ -261,9 +261,10 @@ typedef struct {
  * head_dim, k and v: n_rows rows of n_kv_heads * head_dim.  Rows of out that
  * belong to no sequence keep what they hold.  dtype: F32, F16 or BF16 for all
  * four; scores, softmax and sums are f32 (16-bit types: each weight is rounded
- * to the type for the product with v, and the result once).  A key that a row
- * does not see has no influence on it, whatever it holds.  head_dim: a multiple
- * of 8, at most 256.  Rows have to start at multiples of 16 bytes, strides be
+ * to the type for the product with v, and the result once; f16 weights below
+ * 2^-21 of the row's largest by up to 2^-32 of it).  A key that a row does not
+ * see has no influence on it, whatever it holds.  head_dim: a multiple of 8, at
+ * most 256.  Rows have to start at multiples of 16 bytes, strides be
  * below 2^24 elements, and out be another buffer than the inputs; n_rows *
  * n_heads / n_kv_heads < 2^31.  Offsets past n_rows or decreasing touch nothing
  * outside the buffers, but which rows then hold results is not defined.

@@ -7,7 +7,7 @@
 // read serves every head of the group.  A wave holds 32 slots and walks its keys
 // in subtiles of 32 with an online softmax:
 //   S^T = K Q^T      keys x slots, a lane holds 16 keys of one slot
-//   p = 2^(c S - m), m a running maximum of c S (up to kLag behind), c = log2(e) / sqrt(hd)
+//   p = 2^(c S - m), m a running maximum of c S (up to kLag behind, less kRaise), c = log2(e) / sqrt(hd)
 //   O^T += V^T P^T   dims x slots; the lane's p are the operand as they lie
 // on the 32-row matrix instructions (operand row or column = lane % 32, k from h
 // = lane / 32; result column = lane % 32, row = 8 (i / 4) + 4 h + i % 4).  The
@@ -49,7 +49,11 @@ __device__ __forceinline__ f16v mma16(i4v a, i4v b, f16v c) {
 
 // Eight weights as an operand, rounded to the type: 2^-8 (bf16) or 2^-11 of each at
 // most, as much as the result's own rounding, and of either sign, so that the two
-// together stay below 1.5 times the one.  The weights' sum keeps f32.
+// together stay below 1.5 times the one.  f16 has a fixed step below 2^-14, so that
+// many small weights beside a large one would be off together, and lost below 2^-25
+// (1700 keys of weight 2^-26: all of them), while the sum has them.  They are taken
+// 2^kRaise times as large: off by 2^-32 of the walk's largest weight at most, where
+// that is more than 2^-11 of their own.  The weights' sum keeps f32.
 template <typename T>
 __device__ __forceinline__ i4v pack8(const f16v &s, int at) {
     if constexpr (__is_same(T, _Float16)) {
@@ -169,17 +173,19 @@ __device__ __forceinline__ float max_halves(float x) {
 // What weights are taken against: a running maximum m of c S that lags up to kLag
 // behind the true one, so that the weight's sum l (this lane's keys) and the sums o
 // are rescaled a few times and not with every new maximum of any slot (half of
-// the subtiles of a long walk; a sixth of its time).  Weights reach 2^kLag then:
-// no 16-bit type minds, and what is small is kept better.
+// the subtiles of a long walk; a sixth of its time), and is kRaise below it.
+// Weights reach 2^(kLag + kRaise) then: 2^15 in f16, which ends at 65504.
 constexpr float kLag = 8.f;
-template <uint32_t N, uint32_t DT>
+template <typename T>
+constexpr float kRaise = __is_same(T, _Float16) ? 7.f : 0.f;
+template <typename T, uint32_t N, uint32_t DT>
 __device__ __forceinline__ void new_maximum(const f16v (&s)[N], f16v (&o)[DT], float &m, float &l, float c) {
     float cm = s[0][0];
 #pragma unroll
     for (uint32_t n = 0; n < N; n++)
 #pragma unroll
         for (int i = n ? 0 : 1; i < 16; i++) cm = fmaxf(cm, s[n][i]);
-    cm = max_halves(cm) * c;
+    cm = max_halves(cm) * c - kRaise<T>;
     if (__ballot(cm > m + kLag)) {
         const float mn = fmaxf(m, cm);
         // (m = -inf: nothing was added yet, and the factor multiplies zeros)
@@ -206,9 +212,9 @@ __device__ __forceinline__ void weights(f16v (&s)[N], float m, float &l, float c
         }
     l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
 }
-template <uint32_t N, uint32_t DT>
+template <typename T, uint32_t N, uint32_t DT>
 __device__ __forceinline__ void online_softmax(f16v (&s)[N], f16v (&o)[DT], float &m, float &l, float c) {
-    new_maximum(s, o, m, l, c);
+    new_maximum<T>(s, o, m, l, c);
     weights(s, m, l, c);
 }
 
@@ -220,7 +226,7 @@ struct WaveAttn {
     static constexpr uint32_t LDS = 2 * SUB;   // bytes of a wave that walks by itself
     i4v q[NS];    // bytes 32 s + 16 h .. of this lane's slot's query
     f16v o[DT];   // O^T, unnormalised: dim 32 t + 8 (i / 4) + 4 h + i % 4
-    float m, l;   // running maximum of c S; this lane's share of the weight's sum
+    float m, l;   // what weights are taken against; this lane's share of their sum
 
     __device__ __forceinline__ void init(const uint8_t *qrow, uint32_t hb, uint32_t h) {
 #pragma unroll
@@ -341,7 +347,7 @@ struct WaveAttn {
             wait_lds();
             if (more) copy(K, No{}, key + step);
             if (decltype(masked)::value) hide(s[0], key, lim, lane);
-            online_softmax<1, DT>(s, o, m, l, c);
+            online_softmax<T>(s, o, m, l, c);
             if (more) wait_copies<NL>();   // V is there
             else wait_copies<0>();
             if (decltype(masked)::value) dropped |= drop_not_finite<T, NL>(vt, lane);
@@ -452,7 +458,7 @@ struct WaveAttn<float, D> {
                 copy(key, DT + j);
             }
             if (decltype(masked)::value) WaveAttn<_Float16, D>::hide(s[0], key, lim, lane);
-            online_softmax<1, DT>(s, o, m, l, c);
+            online_softmax<float>(s, o, m, l, c);
 #pragma unroll
             for (uint32_t j = 0; j < DT; j++) {   // O^T += V^T P^T
                 if (more) wait_copies<4 * (DT - 1)>();
@@ -669,7 +675,7 @@ struct TileAttn {
             const uint8_t *kb = uniform(reinterpret_cast<uint64_t>(K.p) + (uint64_t)(key + 2 * STEP) * K.stride);
             const uint8_t *vb = uniform(reinterpret_cast<uint64_t>(V.p) + (uint64_t)(key + STEP) * V.stride);
             const uint32_t kd = lds0 + TILE * (2 * buf), vd = lds0 + TILE * (2 * (buf ^ 1u) + 1);
-            new_maximum(s, w.o, w.m, w.l, c);
+            new_maximum<T>(s, w.o, w.m, w.l, c);
             f16v p[NSUB];
 #pragma unroll
             for (uint32_t n = 0; n < NSUB; n++) p[n] = s[n];
@@ -697,7 +703,7 @@ struct TileAttn {
         };
         for (; key + KEYS <= lim_lo; key += STEP, buf ^= 1u) {   // tiles that every slot of the wave sees whole
             next();
-            new_maximum(s, w.o, w.m, w.l, c);
+            new_maximum<T>(s, w.o, w.m, w.l, c);
             f16v p[NSUB];
 #pragma unroll
             for (uint32_t n = 0; n < NSUB; n++) p[n] = s[n];
@@ -712,7 +718,7 @@ struct TileAttn {
             if (key >= lim_hi) continue;
 #pragma unroll
             for (uint32_t n = 0; n < NSUB; n++) W::hide(s[n], key + 32 * n, lim, lane);
-            new_maximum(s, w.o, w.m, w.l, c);
+            new_maximum<T>(s, w.o, w.m, w.l, c);
             weights(s, w.m, w.l, c);
             const uint32_t ln = opaque(lane) & 63u;
 #pragma unroll
