@@ -298,7 +298,8 @@ int yule_hip_prefix_attn(yule_hip_backend *be, const yule_rows *q, const yule_ro
  * [n_seqs][n_draft]).  target: f32 rows s * (n_draft + 1) + i of vocab
  * probabilities, of the token after i drafts; draft: rows s * n_draft + i, the
  * probabilities that draft i was drawn from; uniforms: f32 [n_seqs][n_draft +
- * 1] numbers in [0, 1).  Draft i is kept while all before it are and
+ * 1] numbers in [0, 1).  vocab is at most 2^30, strides are any that the
+ * buffers hold.  Draft i is kept while all before it are and
  * uniforms[i] * draft_i[x] < target_i[x]; the first that is not, a, is replaced
  * by a token of weights max(target_a - draft_a, 0) (all zero: of target_a), and
  * if all are kept one of target_a follows: the smallest token at which the

@@ -136,3 +136,25 @@ def test_verify_drafts_many_sequences(hip):
     wa, wt = verify_reference(p, q, drafts, u, [n] * b, vocab)
     for acc, tok in got:
         assert np.array_equal(acc, wa) and np.array_equal(tok, wt)
+
+
+def test_verify_drafts_wide_vocabulary(hip):
+    """Rows of 2^24 values and more."""
+    vocab = (1 << 24) + 5
+    say(f"[batch] verify_drafts, {vocab} values")
+    p, q = torch.zeros(4, vocab, device="cuda"), torch.zeros(2, vocab, device="cuda")
+    x = 1 << 24
+    p[0, 3], p[0, x + 4], p[0, x + 1], q[0, x + 1] = .25, .5, .25, .5   # draft x + 1: .75 * .5 >= .25, weights .25 and .5
+    p[2, x + 2], q[1, x + 2] = .5, .5                                   # kept
+    p[3, 64 * 4096 + 7], p[3, x] = .5, .5                               # the sum has to pass .5
+    p[1], p[3, 5] = float("nan"), -1                                    # (not looked at; no weight)
+    ids = torch.tensor([x + 1, x + 2], dtype=torch.int32, device="cuda")
+    u = torch.tensor([[.75, .5], [.75, .5]], device="cuda")
+    acc, tok = (torch.zeros(n, dtype=torch.int32, device="cuda") for n in (2, 4))
+    torch.cuda.synchronize()
+    h = [hip.import_buffer(t.data_ptr(), t.numel() * 4) for t in (p, q, ids, u, acc, tok)]
+    hip.verify_drafts(h[0], h[1], h[2], h[3], None, h[4], h[5], 2, 1, vocab)
+    hip.synchronize()
+    assert acc.tolist() == [0, 1] and tok.tolist() == [x + 4, -1, x + 2, x]
+    for b in h:
+        hip.free(b)

@@ -65,3 +65,39 @@ def test_prefix_shapes(plan, shape, join, p_slots):
         lanes = 16 if hd <= 64 else 32 if hd <= 128 else 64
         threads, ahead = (64, 0) if parts <= 2 * 64 // lanes else (256, 0) if parts <= 4 * 256 // lanes else (256, 8)
         assert (threads, lanes, ahead) == join, (dt, parts)
+
+
+ROWS = r"""
+#include <cstdio>
+#include <initializer_list>
+#include "batch_plan.h"
+using namespace yule;
+#define CHECK(x) do { if (!(x)) { printf("line %d: %s\n", __LINE__, #x); return 1; } } while (0)
+int main() {
+    const uint64_t big = 1ull << 45, far = 1ull << 24;
+    // one row: its stride is never looked at
+    CHECK(!check_rows(0, far, 1, 64, 4, big, 16) && !check_rows(8, ~0ull, 1, 64, 2, big, 16));
+    CHECK(!check_rows(0, far - 4, 2, 64, 4, big, 16) && check_rows(0, far, 2, 64, 4, big, 16));   // attention's limit
+    // rows of probabilities: any stride, a vocabulary's of 2^24 and more among them, inside the buffer
+    for (uint64_t n = 1; n <= 4; n++)
+        for (uint64_t vocab : {far - 1, far, far + 5, (uint64_t)kMaxVocab}) {
+            CHECK(!check_rows(0, vocab, n, vocab, 4, 4 * n * vocab, 4, kAnyStride));
+            CHECK(check_rows(0, vocab, n, vocab, 4, 4 * n * vocab - 4, 4, kAnyStride));
+            CHECK(check_rows(1, vocab, n, vocab, 4, 4 * n * vocab, 4, kAnyStride));
+        }
+    CHECK(check_rows(0, ~0ull, 2, 64, 4, big, 4, kAnyStride) && check_rows(0, 1ull << 62, 2, 64, 4, big, 4, kAnyStride));
+    printf("ok\n");
+    return 0;
+}
+"""
+
+
+def test_strides(tmp_path):
+    gxx = shutil.which("g++")
+    if gxx is None:
+        pytest.skip("no g++")
+    (tmp_path / "t.cpp").write_text(ROWS)
+    subprocess.run([gxx, "-O1", "-std=c++17", "-Wall", "-fsanitize=undefined", "-fno-sanitize-recover", f"-I{CSRC}",
+                    str(tmp_path / "t.cpp"), "-o", str(tmp_path / "t")], check=True)
+    r = subprocess.run([str(tmp_path / "t")], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0 and r.stdout.strip() == "ok", r.stdout + r.stderr

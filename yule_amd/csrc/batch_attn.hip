@@ -1216,7 +1216,7 @@ struct Checked {
 int rows_arg(yule_hip_backend *be, const yule_rows *r, uint64_t n_rows, uint64_t width, uint32_t elem, const char *what,
              Checked *out) {
     void *p;
-    int rc = rows_ptr(be, r, n_rows, width, elem, 16, what, &p);
+    int rc = rows_ptr(be, r, n_rows, width, elem, 16, kMaxAttnStride, what, &p);
     if (rc) return rc;
     out->p = static_cast<uint8_t *>(p);
     out->stride = n_rows > 1 ? (uint32_t)(r->stride * elem) : 0u;   // (one row or none: any stride is given)

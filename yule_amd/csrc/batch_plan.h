@@ -18,22 +18,24 @@ inline uint32_t attn_elem_bytes(uint32_t dtype) {
 }
 
 // the head size that the kernels are built for (dims past head_dim are zeros in
-// registers and LDS); f32: the next multiple of 32, so that every piece of 32
-// dims holds some of the head
+// registers, and zeros in LDS or left out); f32: the next multiple of 32, so that
+// every piece of 32 dims holds some of the head
 inline uint32_t attn_padded_dim(uint32_t hd, uint32_t elem) {
     return elem == 4 ? (hd + 31) / 32 * 32 : hd <= 64 ? 64u : hd <= 96 ? 96u : hd <= 128 ? 128u : 256u;
 }
 
 // Rows r < n_rows, each `width` elements of `elem` bytes, of a buffer of
 // buf_bytes: nullptr, or what is wrong.  align: bytes that every row starts at
-// a multiple of.  Offsets inside a tile (32 rows of f32, 64 of 16-bit types) have
-// to fit 31 bits: the copies into LDS take 32-bit offsets from a 64-bit row address.
+// a multiple of.  max_stride: of several rows, what every stride is below.
+// Attention's: offsets inside a tile (32 rows of f32, 64 of 16-bit types) have to fit
+// 31 bits, as the copies into LDS take 32-bit offsets from a 64-bit row address.
+constexpr uint64_t kMaxAttnStride = (uint64_t)1 << 24, kAnyStride = ~(uint64_t)0;
 inline const char *check_rows(uint64_t offset, uint64_t stride, uint64_t n_rows, uint64_t width, uint32_t elem,
-                              uint64_t buf_bytes, uint32_t align) {
+                              uint64_t buf_bytes, uint32_t align, uint64_t max_stride = kMaxAttnStride) {
     if (!n_rows || !width) return nullptr;
     const uint64_t elems = buf_bytes / elem;
     if (stride < width && n_rows > 1) return "rows overlap (stride below the row's width)";
-    if (stride >= (uint64_t)1 << 24) return "row stride of 2^24 elements or more";
+    if (stride >= max_stride && n_rows > 1) return "row stride of 2^24 elements or more";
     if (width > elems || offset > elems - width) return "rows reach past the buffer";
     if (n_rows > 1 && (elems - width - offset) / stride < n_rows - 1) return "rows reach past the buffer";
     if ((offset * elem) % align || (n_rows > 1 && (stride * elem) % align)) return "rows are not aligned";

@@ -69,9 +69,9 @@ int get_buffer(yule_hip_backend *be, uint64_t h, size_t need, void **ptr, const 
 
 // Rows r < n_rows of an argument of a batched operator, `width` elements of
 // `elem` bytes each: address of the first (align: what every row starts at a
-// multiple of), or the refusal.
+// multiple of; max_stride: what strides are below), or the refusal.
 int rows_ptr(yule_hip_backend *be, const yule_rows *r, uint64_t n_rows, uint64_t width, uint32_t elem, uint32_t align,
-             const char *what, void **ptr);
+             uint64_t max_stride, const char *what, void **ptr);
 
 // A C entry's body: with the backend's device current (the caller's is put
 // back), and with C++ exceptions turned into an error.

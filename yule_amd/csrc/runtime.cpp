@@ -94,13 +94,13 @@ int get_buffer(yule_hip_backend *be, uint64_t h, size_t need, void **ptr, const 
 }
 
 int rows_ptr(yule_hip_backend *be, const yule_rows *r, uint64_t n_rows, uint64_t width, uint32_t elem, uint32_t align,
-             const char *what, void **ptr) {
+             uint64_t max_stride, const char *what, void **ptr) {
     if (!r) return set_error(YULE_ERR_INVALID, std::string(what) + ": null rows");
     std::lock_guard<std::mutex> lk(be->mu);
     auto it = be->buffers.find(r->buffer);
     if (it == be->buffers.end())
         return set_error(YULE_ERR_INVALID, std::string(what) + ": buffer " + std::to_string(r->buffer) + " not found");
-    if (const char *bad = check_rows(r->offset, r->stride, n_rows, width, elem, it->second.size, align))
+    if (const char *bad = check_rows(r->offset, r->stride, n_rows, width, elem, it->second.size, align, max_stride))
         return set_error(YULE_ERR_INVALID, std::string(what) + ": " + bad);
     *ptr = static_cast<uint8_t *>(it->second.ptr) + (n_rows && width ? r->offset * elem : 0);
     return YULE_OK;

@@ -260,8 +260,8 @@ extern "C" int yule_hip_verify_drafts(yule_hip_backend *be, const yule_rows *tar
         VerifyArgs a = {};
         void *pp, *pq = nullptr, *pd = nullptr, *pu, *pl = nullptr, *pa, *pt;
         int rc;
-        if ((rc = rows_ptr(be, target, rows_p, vocab, 4, 4, "verify_drafts (target)", &pp)) ||
-            (n_draft && (rc = rows_ptr(be, draft, rows_q, vocab, 4, 4, "verify_drafts (draft)", &pq))) ||
+        if ((rc = rows_ptr(be, target, rows_p, vocab, 4, 4, kAnyStride, "verify_drafts (target)", &pp)) ||
+            (n_draft && (rc = rows_ptr(be, draft, rows_q, vocab, 4, 4, kAnyStride, "verify_drafts (draft)", &pq))) ||
             (n_draft && (rc = get_buffer(be, draft_tokens, rows_q * 4, &pd, "verify_drafts (draft_tokens)", 0, true))) ||
             (rc = get_buffer(be, uniforms, rows_p * 4, &pu, "verify_drafts (uniforms)", 0, true)) ||
             (draft_lens && (rc = get_buffer(be, draft_lens, (size_t)n_seqs * 4, &pl, "verify_drafts (draft_lens)", 0, true))) ||
