@@ -89,8 +89,8 @@ int guarded(const char *what, yule_hip_backend *be, F body) {
             }
         } back{was, be->device};
         return body();
-    } catch (...) {   // (an allocation of the host's)
-        return YULE_ERR_OOM;
+    } catch (...) {   // an allocation of the host's (and the message's characters need none)
+        return set_error(YULE_ERR_OOM, "out of memory");
     }
 }
 
