@@ -58,17 +58,21 @@ int get_scratch(yule_hip_backend *be, size_t need, ScratchLease *lease) {
         // neither the wait nor the allocation can be captured, and trying would spoil the capture
         if (cap != hipStreamCaptureStatusNone)
             return set_error(YULE_ERR_HIP, "scratch: cannot grow under stream capture");
-        if (be->scratch) {
+        // one that no graph has gives its memory back first; one that stays anyway is used on if there is no larger one
+        if (be->scratch && !be->scratch_in_graph) {
             if ((rc = hip_error(hipStreamSynchronize(be->stream), "scratch: synchronize"))) return rc;
-            if (be->scratch_in_graph) be->scratch_kept.push_back(be->scratch);
-            else (void)hipFree(be->scratch);
+            (void)hipFree(be->scratch);
             be->scratch = nullptr;
             be->scratch_size = 0;
-            be->scratch_in_graph = false;
         }
+        if (be->scratch) be->scratch_kept.reserve(be->scratch_kept.size() + 1);
         const size_t sz = (need + ((size_t)1 << 20) - 1) & ~(((size_t)1 << 20) - 1);
-        if ((rc = workspace_alloc(sz, &be->scratch, "scratch: allocate"))) return rc;
+        void *larger;
+        if ((rc = workspace_alloc(sz, &larger, "scratch: allocate"))) return rc;
+        if (be->scratch) be->scratch_kept.push_back(be->scratch);
+        be->scratch = larger;
         be->scratch_size = sz;
+        be->scratch_in_graph = false;
     }
     if (cap != hipStreamCaptureStatusNone) be->scratch_in_graph = true;
     lease->ptr = be->scratch;
