@@ -266,7 +266,9 @@ typedef struct {
  * see has no influence on it, whatever it holds.  head_dim: a multiple of 8, at
  * most 256.  Rows have to start at multiples of 16 bytes, strides be
  * below 2^24 elements, and out be another buffer than the inputs; n_rows *
- * n_heads / n_kv_heads < 2^31.  Offsets past n_rows or decreasing touch nothing
+ * n_heads / n_kv_heads < 2^31, n_heads at most 4096, and n_rows * n_heads / 32 +
+ * n_seqs * n_kv_heads at most 2^23 (a launch's workgroups).  The kernel is chosen
+ * by n_rows and n_seqs, as the lengths are on the device.  Offsets past n_rows or decreasing touch nothing
  * outside the buffers, but which rows then hold results is not defined.
  * Allocates nothing, and can be captured. */
 int yule_hip_prompt_attn(yule_hip_backend *be, const yule_rows *q, const yule_rows *k, const yule_rows *v,
@@ -281,7 +283,8 @@ int yule_hip_prompt_attn(yule_hip_backend *be, const yule_rows *q, const yule_ro
  * of k_tail and v_tail; tail_lens (u32[n_seqs] on the device) above tail_cap
  * count as tail_cap.  A row that sees nothing gives zeros.  n_tokens above 1 is
  * the step that scores drafted tokens.  prefix_len or tail_cap 0: that part's
- * rows are not looked at and may be null; both at most 2^30.  Types, heads,
+ * rows are not looked at and may be null; both at most 2^30; n_seqs * n_tokens *
+ * n_heads, and the workgroups of the chunks, at most 2^23.  Types, heads,
  * alignment, aliasing and accuracy as for yule_hip_prompt_attn.  The chunks'
  * results lie in the backend's workspace (it does not grow under capture: call
  * once before with the same sizes). */
@@ -309,7 +312,8 @@ int yule_hip_prefix_attn(yule_hip_backend *be, const yule_rows *q, const yule_ro
  * behind it.  Weights that are negative or NaN count as 0 (with none left the
  * new token is YULE_NO_TOKEN); a draft of vocab or more is not kept.  n_draft 0
  * (at most 1024): plain sampling, and draft, draft_tokens are not looked at.
- * Outputs have to be other buffers than the inputs and each other.  Uses the
+ * Outputs have to be other buffers than the inputs and each other; n_seqs *
+ * vocab / 4096, rounded up for each sequence, is at most 2^23.  Uses the
  * backend's workspace, as yule_hip_prefix_attn. */
 int yule_hip_verify_drafts(yule_hip_backend *be, const yule_rows *target, const yule_rows *draft,
                            yule_buffer draft_tokens, yule_buffer uniforms, yule_buffer draft_lens,

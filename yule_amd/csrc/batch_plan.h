@@ -106,7 +106,10 @@ constexpr uint32_t kMaxParts = 1024;
 // whose products take eight times as long: where a sequence's pairs fill its tiles
 // (64 sequences of 8 tokens, 300 + 200 keys: 47 against 68 us), and otherwise
 // up to 128 keys, a subtile a wave, as the prefix shares its tiles between the
-// sequences (64 of 1 token, 300 + 200 keys: 79 against 48).
+// sequences, and one launch is a longer chain for a few of them too (1 token,
+// 32/8x128, 300 + 200 keys: 1 sequence 25.8 us against 16.4, 64 44.1 against 40.4;
+// only near the limit one launch is ahead: 32/4x64, 128 + 64 keys, 2 sequences 9.2
+// against 9.5, 64 9.7 against 13.0).
 struct PrefixPlan {
     bool direct;
     uint32_t p_chunk, n_p;   // keys of a prefix chunk, chunks (0 without a prefix)
@@ -127,7 +130,10 @@ inline PrefixPlan prefix_plan(uint32_t prefix_len, uint32_t tail_cap, uint32_t n
     p.p_slots = elem == 2 && slots > kAttnTileRows ? 128u : kAttnTileRows;
     p.p_tiles = (uint32_t)((slots + p.p_slots - 1) / p.p_slots);
     p.t_tiles = (uint32_t)((n_tokens * group + kAttnTileRows - 1) / kAttnTileRows);
-    // Enough chunks for two workgroups a CU, none below 256 keys (two subtiles of every wave): the tails' fill up to
+    // Enough chunks for two workgroups a CU, none below 256 keys (two subtiles of every wave; with 128, of one, 16-bit
+    // types lose by the longer join, 12.9 -> 15.4 us for 13 sequences of 1 token behind 15001 rows, 17.0 -> 19.0 for 8 of
+    // 5 behind 2048, and f32 gains where there are few sequences, 12.4 -> 10.4 for 2 behind 2048 + 256, and loses for 16
+    // of 300 + 200 keys, 18.9 -> 19.9): the tails' fill up to
     // one a CU, the prefix' the rest, so that the two, which are bound by different things, run side by side (64
     // sequences of up to 1024 rows behind 32768, bf16: 87 us with two of the prefix a CU, 70 so; 16 of up to 300
     // behind 8192, f32: 46 and 36).
