@@ -22,4 +22,14 @@ PREFIXES = [
     # the join by one wave, and by four without loads ahead, over tiles that the prefix shares
     ((8, 2, 256, 700, 40, [40, 1, 0, 17, 33, 39, 2, 20], 2), (256, 64, 0), {F32: 32, F16: 128, BF16: 128}),
     ((8, 2, 64, 1500, 24, [24, 3, 0, 8, 24, 11, 1, 2, 24, 5], 2), (64, 16, 0), {F32: 32, F16: 128, BF16: 128}),
+    ((16, 16, 256, 500, 70, [70 - s % 70 for s in range(64)], 64), (64, 64, 0), {F32: 32, F16: 128, BF16: 128}),
+    # the same over tiles of few pairs; the other head sizes of f32
+    ((4, 2, 64, 4000, 30, [30, 7], 1), (256, 16, 0), {F32: 32, F16: 32, BF16: 32}),
+    ((6, 2, 80, 700, 70, [70, 5], 1), (64, 32, 0), {F32: 32, F16: 32, BF16: 32}),
+    ((2, 1, 152, 600, 20, [20, 7], 1), (256, 64, 0), {F32: 32, F16: 32, BF16: 32}),
+    ((2, 1, 168, 600, 20, [3, 20], 1), (256, 64, 0), {F32: 32, F16: 32, BF16: 32}),
+    ((2, 1, 200, 600, 20, [20, 11], 1), (256, 64, 0), {F32: 32, F16: 32, BF16: 32}),
 ]
+
+# in one launch, the head sizes of f32
+SHORT = [(2, 1, hd, 60, 20, [20, 7], 2) for hd in (32, 80, 128, 168, 200, 256)]

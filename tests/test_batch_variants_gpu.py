@@ -40,7 +40,7 @@ def test_prompt_attn_split(hip, dt, heads, kv, hd, lens, slots, split, bad):
 
 
 @pytest.mark.parametrize("dt", list(TYPES), ids=lambda d: d.name)
-@pytest.mark.parametrize("shape", [s for s, *_ in batch_shapes.PREFIXES], ids=lambda s: "x".join(str(s[i]) for i in (0, 1, 2, 3)))
+@pytest.mark.parametrize("shape", [s for s, *_ in batch_shapes.PREFIXES] + batch_shapes.SHORT, ids=lambda s: "x".join(str(s[i]) for i in (0, 1, 2, 3)))
 @pytest.mark.parametrize("bad", [None, NAN, INF])
 def test_prefix_attn_chunks(hip, dt, shape, bad):
     """bad: one value of V in the prefix' last row, in a tile that the prefix does not fill, which every row sees, and V's rows

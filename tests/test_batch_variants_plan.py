@@ -55,6 +55,12 @@ def test_prompt_shapes(plan, dt, heads, kv, hd, lens, slots, split):
     assert plan(len(lens), sum(lens), heads, kv, hd, elem(dt), CUS) == [slots, split]
 
 
+@pytest.mark.parametrize("heads,kv,hd,prefix,cap,lens,tokens", batch_shapes.SHORT)
+def test_short_shapes(plan, heads, kv, hd, prefix, cap, lens, tokens):
+    for dt in (batch_shapes.F32, batch_shapes.F16):
+        assert plan(prefix, cap, len(lens), tokens, heads, kv, hd, elem(dt), CUS)[0] == 1
+
+
 @pytest.mark.parametrize("shape,join,p_slots", batch_shapes.PREFIXES)
 def test_prefix_shapes(plan, shape, join, p_slots):
     heads, kv, hd, prefix, cap, lens, tokens = shape
