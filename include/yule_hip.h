@@ -263,13 +263,16 @@ typedef struct {
  * four; scores, softmax and sums are f32 (16-bit types: each weight is rounded
  * to the type for the product with v, and the result once; f16 weights below
  * 2^-21 of the row's largest by up to 2^-32 of it).  A key that a row does not
- * see has no influence on it, whatever it holds.  head_dim: a multiple of 8, at
- * most 256.  Rows have to start at multiples of 16 bytes, strides be
- * below 2^24 elements, and out be another buffer than the inputs; n_rows *
- * n_heads / n_kv_heads < 2^31, n_heads at most 4096, and n_rows * n_heads / 32 +
- * n_seqs * n_kv_heads at most 2^23 (a launch's workgroups).  The kernel is chosen
- * by n_rows and n_seqs, as the lengths are on the device.  Offsets past n_rows or decreasing touch nothing
- * outside the buffers, but which rows then hold results is not defined.
+ * see has no influence on it, whatever it holds; of one that it sees, an infinity
+ * in v gives one (a NaN where its weight rounds to 0) in its own dim, and a row
+ * all of whose scores are minus infinity gives zeros.  head_dim: a multiple of 8,
+ * at most 256.  Rows have to start at multiples of 16 bytes, strides be below
+ * 2^24 elements, and out be another buffer than the inputs; n_rows * n_heads /
+ * n_kv_heads < 2^31, n_heads at most 4096, and n_rows * n_heads / 32 + n_seqs *
+ * n_kv_heads at most 2^23 (a launch's workgroups).  The kernel is chosen by
+ * n_rows and n_seqs, as the lengths are on the device.  Offsets past n_rows or
+ * decreasing touch nothing outside the buffers, but which rows then hold results
+ * is not defined.
  * Allocates nothing, and can be captured. */
 int yule_hip_prompt_attn(yule_hip_backend *be, const yule_rows *q, const yule_rows *k, const yule_rows *v,
                          const yule_rows *out, yule_buffer offsets, uint32_t n_seqs, uint32_t n_rows,

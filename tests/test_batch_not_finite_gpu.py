@@ -52,3 +52,25 @@ def test_prefix_attn_seen_not_finite(hip, dt, bad, hd, prefix):
     has[:, dim:heads // kv * hd:hd] = True
     assert same_value(got[has], bad)
     check(got[~has], want[~has], bound[~has], "the others")
+
+
+@pytest.mark.parametrize("dt", list(TYPES), ids=lambda d: d.name)
+@pytest.mark.parametrize("n", [3, 700])
+def test_scores_of_minus_infinity(hip, dt, n):
+    """Keys whose scores are minus infinity weigh nothing; a row that has no others gives zeros."""
+    say(f"[batch] prompt_attn and prefix_attn {dt.name}, {n} rows, scores of minus infinity")
+    heads, kv, hd, none = 2, 1, 64, 2
+    q, k, v = normal(1, (n, heads * hd), dt).abs(), normal(2, (n, hd), dt), normal(3, (n, hd), dt)
+    q = q + 0.5                                   # positive: q . k is minus infinity where k is in one dim
+    want, bound = prompt_reference(q[none:], k[none:], v[none:], [n - none], heads, kv, hd, dt)
+    k[:none, 5] = -float("inf")
+    with Dev(hip) as d:
+        out = d.new(q.numel() * q.element_size())
+        args = d.up(q), d.up(k), d.up(v)
+        hip.prompt_attn(*args, out, d.up(np.array([0, n], np.uint32)), 1, n, heads, kv, hd, dt)
+        got = d.down(out, tuple(q.shape), dt)
+        last = run_prefix(hip, d, q[-1:], k, v, k[:0], v[:0], [0], 0, 1, heads, kv, hd, dt)
+        first = run_prefix(hip, d, q[-1:], k[:none], v[:none], k[:0], v[:0], [0], 0, 1, heads, kv, hd, dt)
+    assert (got[:none] == 0).all() and (first == 0).all()
+    check(got[none:], want, bound, "prompt_attn")
+    check(last, want[-1:], bound[-1:], "prefix_attn")

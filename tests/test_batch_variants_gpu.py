@@ -9,7 +9,7 @@ import torch
 import batch_shapes
 from test_batch_gpu import (TYPES, Dev, check, normal, prefix_inputs, prefix_reference, prompt_reference, run_prefix, run_verify,
                             say, verify_reference)
-from yule_amd.backend import NO_TOKEN
+from yule_amd.backend import NO_TOKEN, YuleGpuError
 
 pytestmark = pytest.mark.gpu
 
@@ -158,3 +158,30 @@ def test_verify_drafts_wide_vocabulary(hip):
     assert acc.tolist() == [0, 1] and tok.tolist() == [x + 4, -1, x + 2, x]
     for b in h:
         hip.free(b)
+
+
+def test_limits(hip):
+    """The most rows that a call takes, and one more."""
+    say("[batch] limits of a launch")
+    most, tokens = 1 << 23, 64
+    q, k, v = (torch.ones(n, 8, dtype=torch.float16, device="cuda") for n in (most + tokens, 1, 1))
+    v[0] = torch.arange(8)
+    out, ints = torch.zeros_like(q), torch.zeros(most + 8, dtype=torch.int32, device="cuda")
+    p, other = torch.ones(most + 8, device="cuda"), torch.zeros(most + 8, dtype=torch.int32, device="cuda")
+    small = torch.zeros(16, 8, dtype=torch.float16, device="cuda")
+    torch.cuda.synchronize()
+    hq, hk, hv, ho, hi, hp, hx, hs = h = [hip.import_buffer(t.data_ptr(), t.numel() * t.element_size())
+                                          for t in (q, k, v, out, ints, p, other, small)]
+    u = hip.upload(np.full(most + 8, .5, np.float32))
+    for n, call in ((most // tokens, lambda n: hip.prefix_attn(hq, hk, hv, 1, None, None, hi, 0, ho, n, tokens, 1, 1, 8, 1)),
+                    (most, lambda n: hip.verify_drafts(hp, None, None, u, None, hi, hx, n, 0, 1)),
+                    (most, lambda n: hip.prompt_attn(hq, hq, hq, hs, hi, n, 10, 1, 1, 8, 1))):
+        with pytest.raises(YuleGpuError) as e:
+            call(n + 1)
+        assert e.value.code == 1 and "too many rows" in str(e.value)
+        if n < most:
+            call(n)
+            hip.synchronize()
+            assert bool((out[:most] == v[0]).all()) and not bool(out[most:].any())
+    for x in (*h, u):
+        hip.free(x)
