@@ -104,7 +104,9 @@ int yule_hip_import_buffer(yule_hip_backend *be, void *ptr, size_t size_bytes, y
 
 /* The backend's stream, a hipStream_t of the HIP runtime that the library is
  * linked to, on which every call enqueues its work: what shares memory with the
- * backend runs on it too, or waits by events.  It ends with the backend. */
+ * backend runs on it too, or waits by events.  Calls may be captured from it into
+ * a graph of the caller's, which is replayed on it (on another stream its calls
+ * would meet the backend's own in the workspace).  It ends with the backend. */
 int yule_hip_stream(yule_hip_backend *be, void **out);
 
 /* ComputeBackend::matmul (lib.rs:26-34): C[m,n] = A[m,k] * B[k,n], f32 row-major */

@@ -191,3 +191,42 @@ def test_null_arguments():
     from yule_amd.backend import load_library
     lib, out = load_library(), C.c_uint64()
     assert lib.yule_hip_import_buffer(None, 16, 16, C.byref(out)) == 1 and lib.yule_hip_stream(None, C.byref(C.c_void_p())) == 1
+
+
+def test_graph_of_the_callers(hip):
+    """torch captures its own work and the operators' into one graph on the backend's stream, and replays it between eager
+    calls that use the same workspace."""
+    say("[import] a graph of torch's")
+    be = HipBackend(0)
+    heads, kv, hd, prefix, cap, tails, tokens, dt = 8, 2, 64, 900, 30, [30, 4, 11], 2, DType.BF16
+    stream = torch.cuda.ExternalStream(be.stream)
+    with torch.cuda.stream(stream):
+        t = [x.cuda() for x in prefix_inputs(5, heads, kv, hd, prefix, cap, tails, tokens, dt)]
+        out, scaled, lens = torch.zeros_like(t[0]), torch.zeros_like(t[0]), ints(tails)
+        other = torch.zeros_like(out)
+        with Imported(be) as imp:
+            q, kp, vp, kt, vt = (imp(x) for x in t)
+            hs, ho, hl, hother = imp(scaled), imp(out), imp(lens), imp(other)
+
+            def step():
+                torch.mul(t[0], 0.5, out=scaled)
+                be.prefix_attn(hs, kp, vp, prefix, kt, vt, hl, cap, ho, len(tails), tokens, heads, kv, hd, dt)
+                out.add_(1)
+
+            step()
+            torch.cuda.current_stream().synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream):
+                step()
+            for i in range(4):
+                t[0].mul_(-1.25)
+                lens.copy_(ints([30 - i, 4 + i, 11]))
+                out.zero_()
+                graph.replay()
+                be.prefix_attn(q, kp, vp, prefix, kt, vt, hl, cap, hother, len(tails), tokens, heads, kv, hd, dt)
+                got = out.clone()
+                step()
+                assert torch.equal(bits_of(got), bits_of(out)) and not torch.equal(got, other)
+            torch.cuda.current_stream().synchronize()
+            del graph
+    be.close()
